@@ -7,9 +7,13 @@ hot path of SNU-VGILab/InstaOrder (Mask2Former's MSDeformAttnPixelDecoder encode
   modules.py          MSDeformAttn (the nn.Module that calls the op)
   encoder.py          the pixel decoder's MSDA encoder stack, detectron2-free
   pixel_decoder.py    MSDeformAttnPixelDecoder around it (input projections, FPN, mask features)
+  layer_ext.py        host side of libenc_hip.so (include/enc_hip.h): operators of the layer around the op
+  layer.py            gated_feed_forward, residual_norm (autograd functions and modules)
   synthetic.py        synthetic inputs of the encoder's shape (bench, tests)
 """
 from .functions import MSDeformAttnFunction, ms_deform_attn_core_pytorch
+from .layer import gated_feed_forward
 from .modules import MSDeformAttn
 
-__all__ = ["MSDeformAttnFunction", "MSDeformAttn", "ms_deform_attn_core_pytorch"]
+__all__ = ["MSDeformAttnFunction", "MSDeformAttn", "ms_deform_attn_core_pytorch",
+           "gated_feed_forward"]

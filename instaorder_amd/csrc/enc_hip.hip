@@ -1,0 +1,98 @@
+// enc_hip.hip -- the operators of a transformer encoder layer around its attention op, for gfx950 (MI355X):
+// the gated feed-forward block, the residual norm, and the orthogonalised update that trains their weights.
+// Hand-written HIP; wave = 64 lanes.  C ABI declared in include/enc_hip.h.
+#include <hip/hip_runtime.h>
+#include <stdarg.h>
+#include <stdint.h>
+#include <stdio.h>
+#include <string.h>
+
+#include <atomic>
+#include <type_traits>
+
+#include "enc_hip.h"
+
+namespace {
+#include "enc_common.inc"
+#include "enc_gemm.inc"
+#include "enc_pack.inc"
+
+// ---------------------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------------------
+// An error some other library left pending on this thread is neither reported as ours nor consumed: a launch has
+// failed when the pending error afterwards is a different one.
+struct Call {
+  const char *who;
+  hipStream_t st;
+  hipError_t pending;
+  Call(const char *w, void *stream) : who(w), st(static_cast<hipStream_t>(stream)), pending(hipPeekAtLastError()) {}
+  int launched() const {
+    const hipError_t e = hipPeekAtLastError();
+    if (e != hipSuccess && e != pending)
+      return fail(ENC_ERR_LAUNCH, "%s: kernel launch failed: %s", who, hipGetErrorString(e));
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    return ENC_OK;
+  }
+};
+
+size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
+uint32_t round8(uint32_t v) { return (v + 7u) & ~7u; }
+uint32_t ceil_div(size_t a, size_t b) { return (uint32_t)((a + b - 1) / b); }
+bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+size_t type_size(int dtype) { return dtype == ENC_F32 ? 4 : 2; }
+bool known_type(int dtype) { return dtype == ENC_F32 || dtype == ENC_BF16 || dtype == ENC_F16; }
+int planes_of(int dtype) { return dtype == ENC_F32 ? 3 : 1; }
+
+// Hands out pieces of the caller's workspace; with base == nullptr it only counts.
+struct Carve {
+  char *base;
+  size_t used = 0;
+  explicit Carve(void *b) : base(static_cast<char *>(b)) {}
+  template <typename T>
+  T *take(size_t n) {
+    T *p = base ? reinterpret_cast<T *>(base + used) : nullptr;
+    used += align256(n * sizeof(T));
+    return p;
+  }
+};
+
+#include "enc_ffn_host.inc"
+
+}  // namespace
+
+extern "C" {
+
+int enc_abi_version(void) { return 1; }
+const char *enc_last_error(void) { return g_err; }
+uint64_t enc_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }
+
+size_t enc_gated_ffn_forward_workspace_bytes(int dtype, int64_t tokens, int64_t width, int64_t hidden, int64_t out_width) {
+  return ffn_workspace(dtype, tokens, width, hidden, out_width, false);
+}
+size_t enc_gated_ffn_backward_workspace_bytes(int dtype, int64_t tokens, int64_t width, int64_t hidden, int64_t out_width) {
+  return ffn_workspace(dtype, tokens, width, hidden, out_width, true);
+}
+
+int enc_gated_ffn_forward(int dtype, int activation, const void *x, int64_t x_stride, const void *w_in, const void *b_in,
+                          const void *w_out, const void *b_out, int64_t tokens, int64_t width, int64_t hidden,
+                          int64_t out_width, void *y, float *pre, void *workspace, size_t workspace_bytes, void *stream) {
+  FfnArgs a = {};
+  a.dtype = dtype, a.act = activation, a.x = x, a.x_stride = x_stride, a.w_in = w_in, a.b_in = b_in, a.w_out = w_out;
+  a.b_out = b_out, a.M = tokens, a.D = width, a.F = hidden, a.O = out_width, a.y = y, a.pre = pre;
+  return ffn_forward(Call("enc_gated_ffn_forward", stream), a, workspace, workspace_bytes);
+}
+
+int enc_gated_ffn_backward(int dtype, int activation, const void *x, int64_t x_stride, const void *w_in,
+                           const void *w_out, const float *pre, const void *grad, int64_t grad_stride, int64_t tokens,
+                           int64_t width, int64_t hidden, int64_t out_width, void *d_x, void *d_w_in, void *d_b_in,
+                           void *d_w_out, void *d_b_out, void *workspace, size_t workspace_bytes, void *stream) {
+  FfnArgs a = {};
+  a.dtype = dtype, a.act = activation, a.x = x, a.x_stride = x_stride, a.w_in = w_in, a.w_out = w_out;
+  a.M = tokens, a.D = width, a.F = hidden, a.O = out_width, a.pre = const_cast<float *>(pre);
+  a.grad = grad, a.grad_stride = grad_stride, a.d_x = d_x, a.d_w_in = d_w_in, a.d_b_in = d_b_in;
+  a.d_w_out = d_w_out, a.d_b_out = d_b_out;
+  return ffn_backward(Call("enc_gated_ffn_backward", stream), a, workspace, workspace_bytes);
+}
+
+}  // extern "C"
