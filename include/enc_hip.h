@@ -62,6 +62,39 @@ int enc_gated_ffn_backward(int dtype, int activation, const void *x, int64_t x_s
                            int64_t width, int64_t hidden, int64_t out_width, void *d_x, void *d_w_in, void *d_b_in,
                            void *d_w_out, void *d_b_out, void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * Residual norm: the norms before and after a block, with the block's gate and residual scale.
+ *   z = norm_inner(y)  (y itself: ENC_NORM_NONE)
+ *   r = x + gate * scale * z
+ *   n = norm_outer(r)
+ *   norm: ENC_NORM_LAYER (v - mean) / sqrt(var + eps) * weight + bias;  ENC_NORM_RMS v / sqrt(mean(v^2) + eps) * weight + bias
+ * x, y [rows, width]; gate NULL or [rows / gate_group, width], row i / gate_group belongs to row i (gate_group 1: a gate
+ * for each row); scale, weights and biases NULL (absent) or [width].  Width at most 16384; rows need no alignment.
+ * residual: r, may be NULL if there is an outer norm; normed: n, not written without one.  stats: NULL, or 4 floats a
+ * row (16-byte aligned) that the backward pass takes.
+ * Backward: d_normed is needed with an outer norm; d_residual may be NULL with one and is needed without.  d_x and d_y
+ * may be NULL.  Any of the others may be NULL; those given are fully written (zeros for no rows).
+ */
+#define ENC_NORM_NONE 0
+#define ENC_NORM_LAYER 1
+#define ENC_NORM_RMS 2
+
+size_t enc_residual_norm_backward_workspace_bytes(int64_t rows, int64_t width, int64_t gate_group);
+
+int enc_residual_norm_forward(int dtype, int inner, int outer, float eps, const void *x, int64_t x_stride, const void *y,
+                              int64_t y_stride, const void *gate, int64_t gate_stride, int64_t gate_group, const void *scale,
+                              const void *inner_weight, const void *inner_bias, const void *outer_weight,
+                              const void *outer_bias, int64_t rows, int64_t width, void *residual, void *normed, float *stats,
+                              void *stream);
+
+int enc_residual_norm_backward(int dtype, int inner, int outer, const void *x, int64_t x_stride, const void *y, int64_t y_stride,
+                               const void *gate, int64_t gate_stride, int64_t gate_group, const void *scale,
+                               const void *inner_weight, const void *inner_bias, const void *outer_weight, const float *stats,
+                               const void *d_residual, int64_t d_residual_stride, const void *d_normed,
+                               int64_t d_normed_stride, int64_t rows, int64_t width, void *d_x, void *d_y, void *d_gate,
+                               void *d_scale, void *d_inner_weight, void *d_inner_bias, void *d_outer_weight,
+                               void *d_outer_bias, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,8 +12,8 @@ hot path of SNU-VGILab/InstaOrder (Mask2Former's MSDeformAttnPixelDecoder encode
   synthetic.py        synthetic inputs of the encoder's shape (bench, tests)
 """
 from .functions import MSDeformAttnFunction, ms_deform_attn_core_pytorch
-from .layer import gated_feed_forward
+from .layer import gated_feed_forward, residual_norm
 from .modules import MSDeformAttn
 
 __all__ = ["MSDeformAttnFunction", "MSDeformAttn", "ms_deform_attn_core_pytorch",
-           "gated_feed_forward"]
+           "gated_feed_forward", "residual_norm"]

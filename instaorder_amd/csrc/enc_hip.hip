@@ -16,6 +16,7 @@ namespace {
 #include "enc_common.inc"
 #include "enc_gemm.inc"
 #include "enc_pack.inc"
+#include "enc_norm.inc"
 
 // ---------------------------------------------------------------------------------------
 // Host side.
@@ -40,7 +41,6 @@ size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
 uint32_t round8(uint32_t v) { return (v + 7u) & ~7u; }
 uint32_t ceil_div(size_t a, size_t b) { return (uint32_t)((a + b - 1) / b); }
 bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-size_t type_size(int dtype) { return dtype == ENC_F32 ? 4 : 2; }
 bool known_type(int dtype) { return dtype == ENC_F32 || dtype == ENC_BF16 || dtype == ENC_F16; }
 int planes_of(int dtype) { return dtype == ENC_F32 ? 3 : 1; }
 
@@ -58,6 +58,7 @@ struct Carve {
 };
 
 #include "enc_ffn_host.inc"
+#include "enc_norm_host.inc"
 
 }  // namespace
 
@@ -93,6 +94,41 @@ int enc_gated_ffn_backward(int dtype, int activation, const void *x, int64_t x_s
   a.grad = grad, a.grad_stride = grad_stride, a.d_x = d_x, a.d_w_in = d_w_in, a.d_b_in = d_b_in;
   a.d_w_out = d_w_out, a.d_b_out = d_b_out;
   return ffn_backward(Call("enc_gated_ffn_backward", stream), a, workspace, workspace_bytes);
+}
+
+size_t enc_residual_norm_backward_workspace_bytes(int64_t rows, int64_t width, int64_t gate_group) {
+  if (check_norm("enc_residual_norm_backward_workspace_bytes", ENC_F32, rows, width, gate_group, NORM_NONE, NORM_NONE)) return 0;
+  return norm_backward_workspace(rows, width, gate_group);
+}
+
+int enc_residual_norm_forward(int dtype, int inner, int outer, float eps, const void *x, int64_t x_stride, const void *y,
+                              int64_t y_stride, const void *gate, int64_t gate_stride, int64_t gate_group, const void *scale,
+                              const void *inner_weight, const void *inner_bias, const void *outer_weight,
+                              const void *outer_bias, int64_t rows, int64_t width, void *residual, void *normed, float *stats,
+                              void *stream) {
+  NormArgs a = {};
+  a.x = x, a.y = y, a.gate = gate, a.scale = scale, a.iw = inner_weight, a.ib = inner_bias, a.ow = outer_weight, a.ob = outer_bias;
+  a.x_ld = (size_t)x_stride, a.y_ld = (size_t)y_stride, a.gate_ld = (size_t)gate_stride;
+  a.inner = inner, a.outer = outer, a.eps = eps, a.residual = residual, a.normed = normed, a.stats = stats;
+  return norm_forward(Call("enc_residual_norm_forward", stream), dtype, rows, width, gate_group, a);
+}
+
+int enc_residual_norm_backward(int dtype, int inner, int outer, const void *x, int64_t x_stride, const void *y, int64_t y_stride,
+                               const void *gate, int64_t gate_stride, int64_t gate_group, const void *scale,
+                               const void *inner_weight, const void *inner_bias, const void *outer_weight, const float *stats,
+                               const void *d_residual, int64_t d_residual_stride, const void *d_normed,
+                               int64_t d_normed_stride, int64_t rows, int64_t width, void *d_x, void *d_y, void *d_gate,
+                               void *d_scale, void *d_inner_weight, void *d_inner_bias, void *d_outer_weight,
+                               void *d_outer_bias, void *workspace, size_t workspace_bytes, void *stream) {
+  NormArgs a = {};
+  a.x = x, a.y = y, a.gate = gate, a.scale = scale, a.iw = inner_weight, a.ib = inner_bias, a.ow = outer_weight;
+  a.x_ld = (size_t)x_stride, a.y_ld = (size_t)y_stride, a.gate_ld = (size_t)gate_stride;
+  a.inner = inner, a.outer = outer, a.stats = const_cast<float *>(stats);
+  a.d_residual = d_residual, a.dr_ld = (size_t)d_residual_stride, a.d_normed = d_normed, a.dn_ld = (size_t)d_normed_stride;
+  a.dx = d_x, a.dy = d_y;
+  void *const sums[5] = {d_scale, d_inner_weight, d_inner_bias, d_outer_weight, d_outer_bias};
+  return norm_backward(Call("enc_residual_norm_backward", stream), dtype, rows, width, gate_group, a, sums, d_gate, workspace,
+                       workspace_bytes);
 }
 
 }  // extern "C"

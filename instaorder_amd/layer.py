@@ -1,6 +1,7 @@
 """Operators of an encoder layer around its attention op, on the kernels of libenc_hip.so (layer_ext.py):
 
     gated_feed_forward(x, w_in, b_in, w_out, b_out, activation)
+    residual_norm(x, y, gate=, scale=, inner=, outer=, ...)
 
 GPU tensors always take the HIP kernels (errors propagate); CPU tensors take an elementary PyTorch path by explicit
 device dispatch, as ``MSDeformAttn`` does."""
@@ -51,3 +52,62 @@ def gated_feed_forward(x, w_in, b_in, w_out, b_out, activation="silu"):
     if _wants_grad(x, w_in, b_in, w_out, b_out):
         return GatedFeedForwardFunction.apply(x, w_in, b_in, w_out, b_out, activation)
     return layer_ext.gated_ffn_forward(x, w_in, b_in, w_out, b_out, activation, False)[0]
+
+
+class ResidualNormFunction(Function):
+    """Saves the inputs and four statistics a row; both rows are formed again in the backward pass."""
+
+    @staticmethod
+    def forward(ctx, x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias, inner, outer, eps, want_residual):
+        residual, normed, stats = layer_ext.residual_norm_forward(
+            x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias, eps, want_residual, True)
+        ctx.inner, ctx.outer = inner, outer
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias, stats)
+        return residual, normed
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_residual, d_normed):
+        x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias, stats = ctx.saved_tensors
+        if d_residual is None and (d_normed is None or ctx.outer is None):
+            return (None,) * 12
+        if ctx.outer is not None and d_normed is None:
+            d_normed = torch.zeros_like(x)
+        grads = layer_ext.residual_norm_backward(x, y, gate, scale, ctx.inner, inner_weight, inner_bias, ctx.outer,
+                                                 outer_weight, outer_bias, stats, d_residual, d_normed,
+                                                 ctx.needs_input_grad[:8])
+        return (*grads, None, None, None, None)
+
+
+def _cpu_norm(v, kind, weight, bias, eps):
+    if kind == "layer":
+        return F.layer_norm(v, v.shape[-1:], weight, bias, eps)
+    v = v * torch.rsqrt(v.float().pow(2).mean(-1, keepdim=True) + eps).to(v.dtype)
+    v = v if weight is None else v * weight
+    return v if bias is None else v + bias
+
+
+def residual_norm(x, y, *, gate=None, scale=None, inner=None, inner_weight=None, inner_bias=None, outer="layer",
+                  outer_weight=None, outer_bias=None, eps=1e-5, want_residual=True):
+    """The norms before and after a block, with the block's gate and residual scale, in one pass over the rows:
+
+        z = norm_inner(y);  residual = x + gate * scale * z;  normed = norm_outer(residual)
+
+    -> (residual or None, normed or None).  x, y [..., width]; inner / outer: None, "layer" or "rms", each with an
+    optional weight and bias [width]; scale [width]; gate of x's shape, or with ones in its last dimensions before the
+    width (x [batch, tokens, width], gate [batch, 1, width]: one gate for a sample).  want_residual=False leaves the
+    residual in registers.  fp32, bf16 or fp16, one type for all; fp32 inside, each result rounded once.  Differentiable
+    once in all eight tensors."""
+    if not x.is_cuda:
+        layer_ext.check_residual_norm(x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias,
+                                      want_residual)
+        z = y if inner is None else _cpu_norm(y, inner, inner_weight, inner_bias, eps)
+        z = z if gate is None else z * gate
+        r = x + (z if scale is None else z * scale)
+        return r if want_residual else None, None if outer is None else _cpu_norm(r, outer, outer_weight, outer_bias, eps)
+    if _wants_grad(x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias):
+        return ResidualNormFunction.apply(x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias, inner, outer,
+                                          eps, want_residual)
+    return layer_ext.residual_norm_forward(x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight,
+                                           outer_bias, eps, want_residual, False)[:2]

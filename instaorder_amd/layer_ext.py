@@ -16,6 +16,8 @@ _lib = None
 
 _I, _L, _Z, _P, _F = ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_float
 
+NORMS = {None: 0, "layer": 1, "rms": 2}
+NORM_MAX_WIDTH = 16384
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"silu": 0, "gelu": 1, "sigmoid": 2, "relu": 3}
 
@@ -34,7 +36,12 @@ def _load():
             ("enc_gated_ffn_forward_workspace_bytes", [_I] + [_L] * 4, _Z),
             ("enc_gated_ffn_backward_workspace_bytes", [_I] + [_L] * 4, _Z),
             ("enc_gated_ffn_forward", [_I, _I, _P, _L] + [_P] * 4 + [_L] * 4 + [_P] * 3 + [_Z, _P], _I),
-            ("enc_gated_ffn_backward", [_I, _I, _P, _L] + [_P] * 4 + [_L] * 5 + [_P] * 6 + [_Z, _P], _I)):
+            ("enc_gated_ffn_backward", [_I, _I, _P, _L] + [_P] * 4 + [_L] * 5 + [_P] * 6 + [_Z, _P], _I),
+            ("enc_residual_norm_backward_workspace_bytes", [_L] * 3, _Z),
+            ("enc_residual_norm_forward",
+             [_I, _I, _I, _F, _P, _L, _P, _L, _P, _L, _L] + [_P] * 5 + [_L, _L] + [_P] * 4, _I),
+            ("enc_residual_norm_backward",
+             [_I, _I, _I, _P, _L, _P, _L, _P, _L, _L] + [_P] * 5 + [_P, _L, _P, _L, _L, _L] + [_P] * 9 + [_Z, _P], _I)):
         f = getattr(lib, name)
         f.argtypes, f.restype = args, res
     if lib.enc_abi_version() != 1:
@@ -169,3 +176,99 @@ def gated_ffn_backward(x, w_in, w_out, pre, grad, activation, needs):
     if rc != 0:
         _raise(lib, "gated_feed_forward backward")
     return outs
+
+
+# ---- residual norm ----------------------------------------------------------------------------
+def check_residual_norm(x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias, want_residual):
+    """(gate's rows, rows of x that share one of them); raises what the operator refuses."""
+    what = "residual_norm"
+    if inner not in NORMS or outer not in NORMS:
+        raise RuntimeError("%s: inner and outer are None, 'layer' or 'rms'" % what)
+    if x.dtype not in DTYPES:
+        raise RuntimeError("%s: not implemented for %s" % (what, x.dtype))
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= NORM_MAX_WIDTH:
+        raise RuntimeError("%s: x must be [..., width] with a width of 1 to %d" % (what, NORM_MAX_WIDTH))
+    if outer is None and not want_residual:
+        raise RuntimeError("%s: without an outer norm the residual is the only result" % what)
+    width = (x.shape[-1],)
+    _same(what, x.device, x.dtype, y=y, gate=gate, scale=scale, inner_weight=inner_weight, inner_bias=inner_bias,
+          outer_weight=outer_weight, outer_bias=outer_bias)
+    _shaped(what, y=(y, tuple(x.shape)), scale=(scale, width), inner_weight=(inner_weight, width),
+            inner_bias=(inner_bias, width), outer_weight=(outer_weight, width), outer_bias=(outer_bias, width))
+    if (inner is None and not (inner_weight is None and inner_bias is None)) or (
+            outer is None and not (outer_weight is None and outer_bias is None)):
+        raise RuntimeError("%s: a weight or bias of a norm that is None" % what)
+    if gate is None:
+        return 1
+    # one row for each row of x, or ones in the last dimensions before the width: those rows share it
+    lead, gl = x.shape[:-1], gate.shape[:-1]
+    if gate.dim() == x.dim() and gate.shape[-1] == x.shape[-1]:
+        k = len(lead)
+        while k and gl[k - 1] == 1:
+            k -= 1
+        if gl[:k] == lead[:k]:
+            group = 1
+            for n in lead[k:]:
+                group *= n
+            return max(group, 1)
+    raise RuntimeError("%s: gate has shape %s; for x of %s it is that, or with ones in the last dimensions before the "
+                       "width (rows that share a gate)" % (what, tuple(gate.shape), tuple(x.shape)))
+
+
+def residual_norm_forward(x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias, eps,
+                          want_residual, keep):
+    """-> (residual or None, normed or None, stats or None)"""
+    group = check_residual_norm(x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias,
+                                want_residual)
+    if not x.is_cuda:
+        raise RuntimeError("Not implemented on the CPU")
+    lib = _load()
+    with _On(x.device) as stream:
+        xr, x_ld = _rows(x)
+        yr, y_ld = _rows(y)
+        gr, g_ld = (None, 0) if gate is None else _rows(gate)
+        scale, inner_weight, inner_bias, outer_weight, outer_bias = (
+            None if t is None else t.contiguous() for t in (scale, inner_weight, inner_bias, outer_weight, outer_bias))
+        rows, width = xr.shape
+        residual = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_residual else None
+        normed = torch.empty(x.shape, dtype=x.dtype, device=x.device) if outer is not None else None
+        stats = torch.empty((rows, 4), dtype=torch.float32, device=x.device) if keep else None
+        rc = lib.enc_residual_norm_forward(
+            DTYPES[x.dtype], NORMS[inner], NORMS[outer], eps, xr.data_ptr(), x_ld, yr.data_ptr(), y_ld, _ptr(gr), g_ld,
+            group, _ptr(scale), _ptr(inner_weight), _ptr(inner_bias), _ptr(outer_weight), _ptr(outer_bias), rows, width,
+            _ptr(residual), _ptr(normed), _ptr(stats), stream)
+    if rc != 0:
+        _raise(lib, "residual_norm")
+    return residual, normed, stats
+
+
+def residual_norm_backward(x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias, stats,
+                           d_residual, d_normed, needs):
+    """-> gradients of (x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias), None where `needs` says
+    False.  Where y is added as it is, x and y have one gradient: the same tensor, as for x + y."""
+    what = "residual_norm backward"
+    group = check_residual_norm(x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias, True)
+    _same(what, x.device, x.dtype, d_residual=d_residual, d_normed=d_normed)
+    lib = _load()
+    with _On(x.device) as stream:
+        xr, x_ld = _rows(x)
+        yr, y_ld = _rows(y)
+        gr, g_ld = (None, 0) if gate is None else _rows(gate)
+        dr, dr_ld = (None, 0) if d_residual is None else _rows(d_residual)
+        dn, dn_ld = (None, 0) if d_normed is None else _rows(d_normed)
+        params = [None if t is None else t.contiguous() for t in (scale, inner_weight, inner_bias, outer_weight)]
+        rows, width = xr.shape
+        new = lambda t, n: torch.empty(t.shape, dtype=t.dtype, device=t.device) if n else None      # noqa: E731
+        plain = gate is None and scale is None and inner is None
+        dx = new(x, needs[0] or (plain and needs[1]))
+        dy = new(y, needs[1] and not plain)
+        outs = [new(t, n) for t, n in zip((gate, scale, inner_weight, inner_bias, outer_weight, outer_bias), needs[2:])]
+        nbytes = lib.enc_residual_norm_backward_workspace_bytes(rows, width, group)
+        ws = _workspace(nbytes, x.device)
+        rc = lib.enc_residual_norm_backward(
+            DTYPES[x.dtype], NORMS[inner], NORMS[outer], xr.data_ptr(), x_ld, yr.data_ptr(), y_ld, _ptr(gr), g_ld, group,
+            *[_ptr(t) for t in params], stats.data_ptr(), _ptr(dr), dr_ld, _ptr(dn), dn_ld, rows, width, _ptr(dx), _ptr(dy),
+            *[_ptr(t) for t in outs], _ptr(ws), nbytes, stream)
+    if rc != 0:
+        _raise(lib, what)
+    return (dx if needs[0] else None, (dx if plain else dy) if needs[1] else None, *outs)
