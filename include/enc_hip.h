@@ -95,6 +95,18 @@ int enc_residual_norm_backward(int dtype, int inner, int outer, const void *x, i
                                void *d_scale, void *d_inner_weight, void *d_inner_bias, void *d_outer_weight,
                                void *d_outer_bias, void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * Orthogonalised update (Newton-Schulz steps of the Muon optimiser), a batch of contiguous matrices [batch, rows, cols]:
+ *   X = update / max(|update|, eps)   (Frobenius norm, summed in 64 bits)
+ *   `steps` times:  A = X X^T;  X = a X + (b A + c A A) X      (on the short side: A = X^T X and X from the left if rows > cols)
+ * out: X in `dtype`; it may be `update` itself.  Iterates keep 24 bits (ENC_F32) or 16 (the 16-bit types).
+ * Limits: steps 1 to 100, batch < 65536, the short side at most 65536.
+ */
+size_t enc_orthogonalize_workspace_bytes(int dtype, int64_t batch, int64_t rows, int64_t cols);
+
+int enc_orthogonalize(int dtype, const void *update, void *out, int64_t batch, int64_t rows, int64_t cols, int steps, float a,
+                      float b, float c, float eps, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,11 +9,14 @@ hot path of SNU-VGILab/InstaOrder (Mask2Former's MSDeformAttnPixelDecoder encode
   pixel_decoder.py    MSDeformAttnPixelDecoder around it (input projections, FPN, mask features)
   layer_ext.py        host side of libenc_hip.so (include/enc_hip.h): operators of the layer around the op
   layer.py            gated_feed_forward, residual_norm (autograd functions and modules)
+  optim.py            orthogonalize and the Muon optimiser for the stack's weight matrices
   synthetic.py        synthetic inputs of the encoder's shape (bench, tests)
 """
 from .functions import MSDeformAttnFunction, ms_deform_attn_core_pytorch
 from .layer import gated_feed_forward, residual_norm
 from .modules import MSDeformAttn
+from .optim import Muon, orthogonalize
 
 __all__ = ["MSDeformAttnFunction", "MSDeformAttn", "ms_deform_attn_core_pytorch",
-           "gated_feed_forward", "residual_norm"]
+           "gated_feed_forward", "residual_norm",
+           "Muon", "orthogonalize"]

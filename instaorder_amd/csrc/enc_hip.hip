@@ -59,6 +59,7 @@ struct Carve {
 
 #include "enc_ffn_host.inc"
 #include "enc_norm_host.inc"
+#include "enc_muon_host.inc"
 
 }  // namespace
 
@@ -128,6 +129,17 @@ int enc_residual_norm_backward(int dtype, int inner, int outer, const void *x, i
   a.dx = d_x, a.dy = d_y;
   void *const sums[5] = {d_scale, d_inner_weight, d_inner_bias, d_outer_weight, d_outer_bias};
   return norm_backward(Call("enc_residual_norm_backward", stream), dtype, rows, width, gate_group, a, sums, d_gate, workspace,
+                       workspace_bytes);
+}
+
+size_t enc_orthogonalize_workspace_bytes(int dtype, int64_t batch, int64_t rows, int64_t cols) {
+  if (check_muon("enc_orthogonalize_workspace_bytes", dtype, batch, rows, cols, 1)) return 0;
+  return muon_room(dtype, (size_t)batch, (size_t)rows, (size_t)cols, nullptr).bytes;
+}
+
+int enc_orthogonalize(int dtype, const void *update, void *out, int64_t batch, int64_t rows, int64_t cols, int steps, float a,
+                      float b, float c, float eps, void *workspace, size_t workspace_bytes, void *stream) {
+  return orthogonalize(Call("enc_orthogonalize", stream), dtype, update, out, batch, rows, cols, steps, a, b, c, eps, workspace,
                        workspace_bytes);
 }
 

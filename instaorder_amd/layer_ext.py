@@ -37,6 +37,8 @@ def _load():
             ("enc_gated_ffn_backward_workspace_bytes", [_I] + [_L] * 4, _Z),
             ("enc_gated_ffn_forward", [_I, _I, _P, _L] + [_P] * 4 + [_L] * 4 + [_P] * 3 + [_Z, _P], _I),
             ("enc_gated_ffn_backward", [_I, _I, _P, _L] + [_P] * 4 + [_L] * 5 + [_P] * 6 + [_Z, _P], _I),
+            ("enc_orthogonalize_workspace_bytes", [_I] + [_L] * 3, _Z),
+            ("enc_orthogonalize", [_I, _P, _P] + [_L] * 3 + [_I] + [_F] * 4 + [_P, _Z, _P], _I),
             ("enc_residual_norm_backward_workspace_bytes", [_L] * 3, _Z),
             ("enc_residual_norm_forward",
              [_I, _I, _I, _F, _P, _L, _P, _L, _P, _L, _L] + [_P] * 5 + [_L, _L] + [_P] * 4, _I),
@@ -272,3 +274,36 @@ def residual_norm_backward(x, y, gate, scale, inner, inner_weight, inner_bias, o
     if rc != 0:
         _raise(lib, what)
     return (dx if needs[0] else None, (dx if plain else dy) if needs[1] else None, *outs)
+
+
+# ---- orthogonalised update --------------------------------------------------------------------
+def check_orthogonalize(update, steps):
+    what = "orthogonalize"
+    if update.dtype not in DTYPES:
+        raise RuntimeError("%s: not implemented for %s" % (what, update.dtype))
+    if update.dim() < 2 or min(update.shape[-2:]) < 1:
+        raise RuntimeError("%s: update must be [..., rows, cols] with at least one of each" % what)
+    if not 1 <= steps <= 100:
+        raise RuntimeError("%s: steps must be 1 to 100" % what)
+
+
+def orthogonalize(update, steps, coefficients, eps):
+    """-> a new tensor of update's shape and dtype"""
+    check_orthogonalize(update, steps)
+    if not update.is_cuda:
+        raise RuntimeError("Not implemented on the CPU")
+    lib = _load()
+    a, b, c = coefficients
+    with _On(update.device) as stream:
+        update = update.contiguous()
+        out = torch.empty_like(update)
+        rows, cols = update.shape[-2:]
+        batch = update.numel() // (rows * cols)
+        code = DTYPES[update.dtype]
+        nbytes = lib.enc_orthogonalize_workspace_bytes(code, batch, rows, cols)
+        ws = _workspace(nbytes, update.device)
+        rc = lib.enc_orthogonalize(code, update.data_ptr(), out.data_ptr(), batch, rows, cols, steps, a, b, c, eps, _ptr(ws),
+                                   nbytes, stream)
+    if rc != 0:
+        _raise(lib, "orthogonalize")
+    return out
