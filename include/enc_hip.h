@@ -45,13 +45,15 @@ uint64_t enc_launch_count(void);
  *   [a | b] = x W_in^T + b_in        x [tokens, width], w_in [2 * hidden, width], b_in [2 * hidden] or NULL
  *   h = a * act(b)                   a: the first `hidden` columns (value), b: the others (gate), the order of F.glu
  *   y = h W_out^T + b_out            w_out [out_width, hidden], b_out [out_width] or NULL, y [tokens, out_width]
- * Weights are contiguous.  `pre`: NULL, or [tokens, 2 * round_up(hidden, 8)] floats that the backward pass takes
- * (a in the first half of a row, b in the second).
+ * Weights are contiguous.  `pre`: NULL, or enc_gated_ffn_pre_floats(tokens, hidden) floats (16-byte aligned) that the
+ * backward pass takes: a and b in fp32, in the library's own order.
  * Backward: `grad` = gradient of y.  Any of the five results may be NULL; the others are fully written.
  * Limits: every size < 2^22, tokens < 2^31 / 256.
  */
 size_t enc_gated_ffn_forward_workspace_bytes(int dtype, int64_t tokens, int64_t width, int64_t hidden, int64_t out_width);
 size_t enc_gated_ffn_backward_workspace_bytes(int dtype, int64_t tokens, int64_t width, int64_t hidden, int64_t out_width);
+
+size_t enc_gated_ffn_pre_floats(int64_t tokens, int64_t hidden);
 
 int enc_gated_ffn_forward(int dtype, int activation, const void *x, int64_t x_stride, const void *w_in, const void *b_in,
                           const void *w_out, const void *b_out, int64_t tokens, int64_t width, int64_t hidden,

@@ -76,6 +76,10 @@ size_t enc_gated_ffn_backward_workspace_bytes(int dtype, int64_t tokens, int64_t
   return ffn_workspace(dtype, tokens, width, hidden, out_width, true);
 }
 
+size_t enc_gated_ffn_pre_floats(int64_t tokens, int64_t hidden) {
+  return tokens < 0 || hidden <= 0 || hidden >= MAX_SIZE ? 0 : pre_floats(tokens, hidden);
+}
+
 int enc_gated_ffn_forward(int dtype, int activation, const void *x, int64_t x_stride, const void *w_in, const void *b_in,
                           const void *w_out, const void *b_out, int64_t tokens, int64_t width, int64_t hidden,
                           int64_t out_width, void *y, float *pre, void *workspace, size_t workspace_bytes, void *stream) {

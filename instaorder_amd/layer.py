@@ -59,7 +59,7 @@ class ResidualNormFunction(Function):
 
     @staticmethod
     def forward(ctx, x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias, inner, outer, eps, want_residual):
-        residual, normed, stats = layer_ext.residual_norm_forward(
+        residual, normed, stats, ctx.group = layer_ext.residual_norm_forward(
             x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias, eps, want_residual, True)
         ctx.inner, ctx.outer = inner, outer
         ctx.set_materialize_grads(False)
@@ -75,8 +75,8 @@ class ResidualNormFunction(Function):
         if ctx.outer is not None and d_normed is None:
             d_normed = torch.zeros_like(x)
         grads = layer_ext.residual_norm_backward(x, y, gate, scale, ctx.inner, inner_weight, inner_bias, ctx.outer,
-                                                 outer_weight, outer_bias, stats, d_residual, d_normed,
-                                                 ctx.needs_input_grad[:8])
+                                                 outer_weight, outer_bias, stats, ctx.group, d_residual, d_normed,
+                                                 ctx.needs_input_grad)
         return (*grads, None, None, None, None)
 
 
