@@ -15,6 +15,7 @@
 namespace {
 #include "enc_common.inc"
 #include "enc_gemm.inc"
+#include "enc_skinny.inc"
 #include "enc_pack.inc"
 #include "enc_norm.inc"
 
