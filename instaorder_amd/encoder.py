@@ -20,6 +20,8 @@ import torch.nn.functional as F
 from torch import nn
 from torch.nn.init import normal_
 
+from . import layer_ext
+from .layer import ACTIVATIONS, gated_feed_forward, residual_norm
 from .modules import MSDeformAttn
 
 
@@ -50,8 +52,13 @@ class PositionEmbeddingSine(nn.Module):
         return torch.cat((pos_y, pos_x), dim=3).permute(0, 3, 1, 2)
 
 
+# Activations of the feed-forward block that take a value and a gate: linear1 is twice as wide, its first half the value
+# (the order of F.glu).  In the reference "glu" halves the hidden width under linear2 and cannot run; here it does.
+GATED = {"glu": "sigmoid", "swiglu": "silu", "geglu": "gelu", "reglu": "relu"}
+
+
 def _activation(name):
-    return {"relu": F.relu, "gelu": F.gelu, "glu": F.glu}[name]
+    return {"relu": F.relu, "gelu": F.gelu, **{k: ACTIVATIONS[v] for k, v in GATED.items()}}[name]
 
 
 class MSDeformAttnTransformerEncoderLayer(nn.Module):
@@ -61,12 +68,15 @@ class MSDeformAttnTransformerEncoderLayer(nn.Module):
         self.self_attn = MSDeformAttn(d_model, n_levels, n_heads, n_points)
         self.dropout1 = nn.Dropout(dropout)
         self.norm1 = nn.LayerNorm(d_model)
-        self.linear1 = nn.Linear(d_model, d_ffn)
+        self.gate = GATED.get(activation)           # name of the gate's activation, None for a plain block
+        self.linear1 = nn.Linear(d_model, 2 * d_ffn if self.gate else d_ffn)
         self.activation = _activation(activation)
         self.dropout2 = nn.Dropout(dropout)
         self.linear2 = nn.Linear(d_ffn, d_model)
         self.dropout3 = nn.Dropout(dropout)
         self.norm2 = nn.LayerNorm(d_model)
+        # opt-in (not reference behaviour): src + block and its norm in one kernel (residual_norm)
+        self.fused_norm = False
         self.use_adapters, self.adapter_scale = use_adapters, adapter_scale
         if use_adapters:        # InstaFormer's trainable adapters (msdeformattn.py:155-166)
             self.adapter = nn.Sequential(nn.Linear(d_model, adapter_dim), nn.ReLU(),
@@ -76,13 +86,29 @@ class MSDeformAttnTransformerEncoderLayer(nn.Module):
             nn.init.zeros_(self.adapter[2].weight)
             nn.init.zeros_(self.adapter[2].bias)
 
+    def _add_and_norm(self, src, block, norm):
+        if (self.fused_norm and src.is_cuda and src.dtype in layer_ext.DTYPES
+                and src.dtype == block.dtype == norm.weight.dtype and src.shape[-1] <= layer_ext.NORM_MAX_WIDTH):
+            return residual_norm(src, block, outer="layer", outer_weight=norm.weight, outer_bias=norm.bias, eps=norm.eps,
+                                 want_residual=False)[1]
+        return norm(src + block)
+
+    def _feed_forward(self, src):
+        if not self.gate:
+            return self.linear2(self.dropout2(self.activation(self.linear1(src))))
+        dropping = self.training and self.dropout2.p > 0
+        if dropping or src.dtype not in layer_ext.DTYPES or src.dtype != self.linear1.weight.dtype:
+            value, gate = self.linear1(src).chunk(2, -1)
+            return self.linear2(self.dropout2(value * self.activation(gate)))
+        return gated_feed_forward(src, self.linear1.weight, self.linear1.bias, self.linear2.weight, self.linear2.bias,
+                                  self.gate)
+
     def forward(self, src, pos, reference_points, spatial_shapes, level_start_index, padding_mask=None):
         query = src if pos is None else src + pos
-        src = self.norm1(src + self.dropout1(self.self_attn(
-            query, reference_points, src, spatial_shapes, level_start_index, padding_mask)))
+        src = self._add_and_norm(src, self.dropout1(self.self_attn(
+            query, reference_points, src, spatial_shapes, level_start_index, padding_mask)), self.norm1)
         side = self.adapter(src) if self.use_adapters else None
-        ffn = self.linear2(self.dropout2(self.activation(self.linear1(src))))
-        src = self.norm2(src + self.dropout3(ffn))
+        src = self._add_and_norm(src, self.dropout3(self._feed_forward(src)), self.norm2)
         if side is not None:
             src = src + self.adapter_scale * side
         return src

@@ -13,7 +13,7 @@ from torch.autograd.function import once_differentiable
 
 from . import layer_ext
 
-_ACT = {"silu": F.silu, "gelu": F.gelu, "sigmoid": torch.sigmoid, "relu": F.relu}
+ACTIVATIONS = {"silu": F.silu, "gelu": F.gelu, "sigmoid": torch.sigmoid, "relu": F.relu}
 
 
 def _wants_grad(*tensors):
@@ -44,11 +44,12 @@ def gated_feed_forward(x, w_in, b_in, w_out, b_out, activation="silu"):
     x [..., width]; w_in [2 * hidden, width] (value rows first, then gate rows -- the order of ``F.glu``); w_out
     [out_width, hidden]; biases may be None.  activation: "silu", "gelu" (by the error function), "sigmoid", "relu".
     fp32, bf16 or fp16, one type for all; sums are fp32, h is rounded to the type once.  Differentiable once in all five
-    tensors.  fp32: an Inf among the inputs gives NaN (its parts multiply zeros), a NaN stays one."""
+    tensors.  fp32 above 64 tokens and in the backward pass: an Inf among the inputs gives NaN (its parts multiply zeros), a
+    NaN stays one, and values below 2^-110 lose their low bits (their parts end at 2^-133)."""
     if not x.is_cuda:
         layer_ext.check_gated_ffn(x, w_in, b_in, w_out, b_out, activation)
         a, b = F.linear(x, w_in, b_in).chunk(2, -1)
-        return F.linear(a * _ACT[activation](b), w_out, b_out)
+        return F.linear(a * ACTIVATIONS[activation](b), w_out, b_out)
     if _wants_grad(x, w_in, b_in, w_out, b_out):
         return GatedFeedForwardFunction.apply(x, w_in, b_in, w_out, b_out, activation)
     return layer_ext.gated_ffn_forward(x, w_in, b_in, w_out, b_out, activation, False)[0]

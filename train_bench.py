@@ -28,19 +28,31 @@ import torch
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from instaorder_amd import distributed as D                      # noqa: E402
 from instaorder_amd import synthetic                              # noqa: E402
+from instaorder_amd import Muon                                   # noqa: E402
 from instaorder_amd.encoder import MSDeformAttnTransformerEncoderOnly, PositionEmbeddingSine  # noqa: E402
 
 
-def build_encoder(levels=3, freeze_base=True, seed=0):
+def build_encoder(levels=3, freeze_base=True, seed=0, activation="relu"):
     torch.manual_seed(seed)
     enc = MSDeformAttnTransformerEncoderOnly(d_model=256, nhead=8, num_encoder_layers=6,
-                                             dim_feedforward=1024, dropout=0.0,
+                                             dim_feedforward=1024, dropout=0.0, activation=activation,
                                              num_feature_levels=levels, enc_n_points=4,
                                              use_adapters=True)
     if freeze_base:
         for name, p in enc.named_parameters():
             p.requires_grad_("adapter" in name)
     return enc
+
+
+def optimisers(enc, name):
+    """AdamW for all that trains, or Muon for its weight matrices and AdamW for the rest (biases, norms, level
+    embeddings)."""
+    train = [(n, p) for n, p in enc.named_parameters() if p.requires_grad]
+    if name == "adamw":
+        return [torch.optim.AdamW([p for _, p in train], lr=1e-4)]
+    matrices = [p for n, p in train if p.dim() == 2 and not n.endswith("level_embed")]
+    rest = [p for n, p in train if p.dim() != 2 or n.endswith("level_embed")]
+    return ([Muon(matrices, lr=2e-3)] if matrices else []) + ([torch.optim.AdamW(rest, lr=1e-4)] if rest else [])
 
 
 def launch_ranks(args):
@@ -65,16 +77,20 @@ def run(args):
     world, rank, local = D.init("gloo" if args.cpu else None)
     device = torch.device("cuda", local) if torch.cuda.is_available() and not args.cpu else torch.device("cpu")
     shapes = synthetic.encoder_shapes(args.image)
-    enc = build_encoder(len(shapes), args.freeze_base).to(device)
+    enc = build_encoder(len(shapes), args.freeze_base, activation=args.activation).to(device)
     if args.fused:      # row f3: softmax + sampling-location arithmetic inside the MSDA kernels
         for mod in enc.modules():
             if hasattr(mod, "fused_prologue"):
                 mod.fused_prologue = True
+    if args.fused_norm:     # src + block and its LayerNorm in one kernel
+        for mod in enc.modules():
+            if hasattr(mod, "fused_norm"):
+                mod.fused_norm = True
     model = enc
     if world > 1:
         from torch.nn.parallel import DistributedDataParallel as DDP
         model = DDP(enc, device_ids=[local] if device.type == "cuda" else None)
-    opt = torch.optim.AdamW([p for p in enc.parameters() if p.requires_grad], lr=1e-4)
+    opts = optimisers(enc, args.optimizer)
     lo, hi = D.shard_batch(args.global_batch, world, rank)
     g = torch.Generator().manual_seed(1234)
     feats = [torch.randn((args.global_batch, 256, h, w), generator=g)[lo:hi].to(device) for h, w in shapes]
@@ -82,11 +98,13 @@ def run(args):
     pos = [pe(x) for x in feats]
 
     def step():
-        opt.zero_grad(set_to_none=True)
+        for opt in opts:
+            opt.zero_grad(set_to_none=True)
         memory, _, _ = model(feats, pos)
         loss = memory.float().pow(2).mean()
         loss.backward()
-        opt.step()
+        for opt in opts:
+            opt.step()
         return loss
 
     for _ in range(args.warmup):
@@ -106,6 +124,7 @@ def run(args):
                                    "%d^2 input, levels %s, global batch %d, %s"
                                    % (args.image, "/".join("%dx%d" % s for s in shapes), args.global_batch,
                                       "adapters only trainable" if args.freeze_base else "all trainable"),
+                       "activation": args.activation, "optimizer": args.optimizer, "fused_norm": args.fused_norm,
                        "device": device.type, "final_loss": float(loss.detach())}}), flush=True)
     D.shutdown()
 
@@ -121,4 +140,8 @@ if __name__ == "__main__":
     ap.add_argument("--all-trainable", dest="freeze_base", action="store_false")
     ap.add_argument("--fused", action="store_true",
                     help="MSDeformAttn.fused_prologue: the fused entry points (SURVEY section 8, row f3)")
+    ap.add_argument("--fused-norm", action="store_true", help="residual add and LayerNorm in one kernel (residual_norm)")
+    ap.add_argument("--activation", default="relu", choices=["relu", "gelu", "glu", "swiglu", "geglu", "reglu"],
+                    help="of the feed-forward block; the last four are gated (gated_feed_forward)")
+    ap.add_argument("--optimizer", default="adamw", choices=["adamw", "muon"])
     run(ap.parse_args())
