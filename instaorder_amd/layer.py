@@ -1,41 +1,16 @@
-"""Operators of an encoder layer around its attention op, on the kernels of libenc_hip.so (layer_ext.py):
+"""Operators of an encoder layer around its attention op, on the kernels of libenc_hip.so:
 
     gated_feed_forward(x, w_in, b_in, w_out, b_out, activation)
     residual_norm(x, y, gate=, scale=, inner=, outer=, ...)
 
-GPU tensors always take the HIP kernels (errors propagate); CPU tensors take an elementary PyTorch path by explicit
-device dispatch, as ``MSDeformAttn`` does."""
+GPU tensors always take the HIP kernels (errors propagate; the autograd nodes are in csrc/enc_bind.cpp); CPU tensors take
+an elementary PyTorch path by explicit device dispatch, as ``MSDeformAttn`` does."""
 import torch
 import torch.nn.functional as F
-from torch import nn
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import layer_ext
 
 ACTIVATIONS = {"silu": F.silu, "gelu": F.gelu, "sigmoid": torch.sigmoid, "relu": F.relu}
-
-
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-class GatedFeedForwardFunction(Function):
-    """Saves x, the two weights and the pre-activations in fp32 (8 bytes a hidden value, what a 16-bit eager block
-    keeps in four tensors), so that the gradients are formed from unrounded values."""
-
-    @staticmethod
-    def forward(ctx, x, w_in, b_in, w_out, b_out, activation):
-        y, pre = layer_ext.gated_ffn_forward(x, w_in, b_in, w_out, b_out, activation, True)
-        ctx.activation = activation
-        ctx.save_for_backward(x, w_in, w_out, pre)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        x, w_in, w_out, pre = ctx.saved_tensors
-        return (*layer_ext.gated_ffn_backward(x, w_in, w_out, pre, grad, ctx.activation, ctx.needs_input_grad[:5]), None)
 
 
 def gated_feed_forward(x, w_in, b_in, w_out, b_out, activation="silu"):
@@ -46,39 +21,12 @@ def gated_feed_forward(x, w_in, b_in, w_out, b_out, activation="silu"):
     fp32, bf16 or fp16, one type for all; sums are fp32, h is rounded to the type once.  Differentiable once in all five
     tensors.  fp32 above 64 tokens and in the backward pass: an Inf among the inputs gives NaN (its parts multiply zeros), a
     NaN stays one, and values below 2^-110 lose their low bits (their parts end at 2^-133)."""
-    if not x.is_cuda:
-        layer_ext.check_gated_ffn(x, w_in, b_in, w_out, b_out, activation)
-        a, b = F.linear(x, w_in, b_in).chunk(2, -1)
-        return F.linear(a * ACTIVATIONS[activation](b), w_out, b_out)
-    if _wants_grad(x, w_in, b_in, w_out, b_out):
-        return GatedFeedForwardFunction.apply(x, w_in, b_in, w_out, b_out, activation)
-    return layer_ext.gated_ffn_forward(x, w_in, b_in, w_out, b_out, activation, False)[0]
-
-
-class ResidualNormFunction(Function):
-    """Saves the inputs and four statistics a row; both rows are formed again in the backward pass."""
-
-    @staticmethod
-    def forward(ctx, x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias, inner, outer, eps, want_residual):
-        residual, normed, stats, ctx.group = layer_ext.residual_norm_forward(
-            x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias, eps, want_residual, True)
-        ctx.inner, ctx.outer = inner, outer
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias, stats)
-        return residual, normed
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_residual, d_normed):
-        x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias, stats = ctx.saved_tensors
-        if d_residual is None and (d_normed is None or ctx.outer is None):
-            return (None,) * 12
-        if ctx.outer is not None and d_normed is None:
-            d_normed = torch.zeros_like(x)
-        grads = layer_ext.residual_norm_backward(x, y, gate, scale, ctx.inner, inner_weight, inner_bias, ctx.outer,
-                                                 outer_weight, outer_bias, stats, ctx.group, d_residual, d_normed,
-                                                 ctx.needs_input_grad)
-        return (*grads, None, None, None, None)
+    bind = layer_ext._bind or layer_ext.bind()
+    if x.is_cuda:
+        return bind.gated_feed_forward(x, w_in, b_in, w_out, b_out, activation)
+    bind.check_gated_feed_forward(x, w_in, b_in, w_out, b_out, activation)
+    a, b = F.linear(x, w_in, b_in).chunk(2, -1)
+    return F.linear(a * ACTIVATIONS[activation](b), w_out, b_out)
 
 
 def _cpu_norm(v, kind, weight, bias, eps):
@@ -100,15 +48,12 @@ def residual_norm(x, y, *, gate=None, scale=None, inner=None, inner_weight=None,
     width (x [batch, tokens, width], gate [batch, 1, width]: one gate for a sample).  want_residual=False leaves the
     residual in registers.  fp32, bf16 or fp16, one type for all; fp32 inside, each result rounded once.  Differentiable
     once in all eight tensors."""
-    if not x.is_cuda:
-        layer_ext.check_residual_norm(x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias,
-                                      want_residual)
-        z = y if inner is None else _cpu_norm(y, inner, inner_weight, inner_bias, eps)
-        z = z if gate is None else z * gate
-        r = x + (z if scale is None else z * scale)
-        return r if want_residual else None, None if outer is None else _cpu_norm(r, outer, outer_weight, outer_bias, eps)
-    if _wants_grad(x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias):
-        return ResidualNormFunction.apply(x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias, inner, outer,
-                                          eps, want_residual)
-    return layer_ext.residual_norm_forward(x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight,
-                                           outer_bias, eps, want_residual, False)[:2]
+    bind = layer_ext._bind or layer_ext.bind()
+    if x.is_cuda:
+        return bind.residual_norm(x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias, eps,
+                                  want_residual)
+    bind.check_residual_norm(x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias, want_residual)
+    z = y if inner is None else _cpu_norm(y, inner, inner_weight, inner_bias, eps)
+    z = z if gate is None else z * gate
+    r = x + (z if scale is None else z * scale)
+    return r if want_residual else None, None if outer is None else _cpu_norm(r, outer, outer_weight, outer_bias, eps)

@@ -12,10 +12,10 @@ def orthogonalize(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     """The nearly orthogonal matrix that `steps` Newton-Schulz steps X <- a X + (b A + c A A) X, A = X X^T, make of
     update / max(|update|, eps) (Frobenius norm).  update [..., rows, cols], a batch of matrices of any shape, fp32, bf16
     or fp16; the result has its shape and type.  Not differentiable.  A zero update gives zeros."""
-    if update.is_cuda:
-        return layer_ext.orthogonalize(update, steps, coefficients, eps)
-    layer_ext.check_orthogonalize(update, steps)
     a, b, c = coefficients
+    if update.is_cuda:
+        return layer_ext.bind().orthogonalize(update, steps, a, b, c, eps)
+    layer_ext.bind().check_orthogonalize(update, steps)
     x = update.float()
     tall = x.shape[-2] > x.shape[-1]
     x = x.mT if tall else x

@@ -574,3 +574,26 @@ def test_encoder_stack_trains_with_muon():
     assert layer_ext.launch_count() > before
     assert all(p.isfinite().all() for p in enc.parameters())
     assert all(not torch.equal(p, w) for p, w in zip(enc.parameters(), weights) if p.grad is not None and p.grad.count_nonzero())
+
+
+def test_gradients_are_differentiable_once():
+    """With create_graph the first gradients are there; differentiating those again is an error, not silence."""
+    from instaorder_amd import gated_feed_forward, residual_norm
+    args = [a.requires_grad_(True) for a in ffn_inputs(torch.float32, 5, 16, 8, 16, True)]
+    for y in (gated_feed_forward(*args), residual_norm(args[0], args[0] * 2, outer="rms")[1]):
+        dx, = torch.autograd.grad(y.square().sum(), args[0], create_graph=True)
+        assert dx.isfinite().all()
+        with pytest.raises(RuntimeError):             # nothing leads from dx back to x
+            torch.autograd.grad(dx.sum(), args[0], retain_graph=True)
+        with pytest.raises(RuntimeError, match="twice"):
+            dx.sum().backward()
+
+
+def test_inputs_changed_after_the_forward_pass_are_noticed():
+    from instaorder_amd import gated_feed_forward
+    args = [a.requires_grad_(True) for a in ffn_inputs(torch.float32, 5, 16, 8, 16, True)]
+    y = gated_feed_forward(*args)
+    with torch.no_grad():
+        args[1].mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()

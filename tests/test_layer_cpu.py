@@ -18,15 +18,30 @@ LIB = os.path.join(ROOT, "instaorder_amd", "libenc_hip.so")
 HEADER = os.path.join(ROOT, "include", "enc_hip.h")
 
 
+I, L, Z, P, F = ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_float
+PROTOTYPES = {
+    "enc_abi_version": ([], I), "enc_last_error": ([], ctypes.c_char_p), "enc_launch_count": ([], ctypes.c_uint64),
+    "enc_gated_ffn_forward_workspace_bytes": ([I] + [L] * 4, Z), "enc_gated_ffn_backward_workspace_bytes": ([I] + [L] * 4, Z),
+    "enc_gated_ffn_pre_floats": ([L, L], Z), "enc_residual_norm_backward_workspace_bytes": ([L] * 3, Z),
+    "enc_orthogonalize_workspace_bytes": ([I] + [L] * 3, Z),
+    "enc_gated_ffn_forward": ([I, I, P, L] + [P] * 4 + [L] * 4 + [P] * 3 + [Z, P], I),
+    "enc_gated_ffn_backward": ([I, I, P, L] + [P] * 4 + [L] * 5 + [P] * 6 + [Z, P], I),
+    "enc_residual_norm_forward": ([I, I, I, F, P, L, P, L, P, L, L] + [P] * 5 + [L, L] + [P] * 4, I),
+    "enc_residual_norm_backward": ([I, I, I, P, L, P, L, P, L, L] + [P] * 6 + [L, P, L, L, L] + [P] * 9 + [Z, P], I),
+    "enc_orthogonalize": ([I, P, P] + [L] * 3 + [I] + [F] * 4 + [P, Z, P], I)}
+
+
 def lib():
-    from instaorder_amd import layer_ext
-    return layer_ext._load()
+    handle = ctypes.CDLL(LIB)
+    for name, (args, res) in PROTOTYPES.items():
+        getattr(handle, name).argtypes, getattr(handle, name).restype = args, res
+    return handle
 
 
 def test_library_exports_every_declared_symbol():
     text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
     names = sorted(set(re.findall(r"\b(enc_[a-z0-9_]+)\s*\(", text)))
-    assert len(names) >= 11
+    assert names == sorted(PROTOTYPES)
     handle = ctypes.CDLL(LIB)
     for n in names:
         assert hasattr(handle, n), n
@@ -130,8 +145,9 @@ def test_python_refusals():
         with pytest.raises(RuntimeError):
             call()
             pytest.fail("call %d was taken" % i)
-    for call in (lambda: layer_ext.gated_ffn_forward(x, wi, bi, wo, bo, "silu", False), lambda: layer_ext.orthogonalize(x, 5, (1, 1, 1), 1.),
-                 lambda: layer_ext.residual_norm_forward(x, x, None, None, None, None, None, "layer", None, None, 1e-5, True, False)):
+    b = layer_ext.bind()                               # the kernels themselves never take a CPU tensor
+    for call in (lambda: b.gated_feed_forward(x, wi, bi, wo, bo, "silu"), lambda: b.orthogonalize(x, 5, 1., 1., 1., 1.),
+                 lambda: b.residual_norm(x, x, None, None, None, None, None, "layer", None, None, 1e-5, True)):
         with pytest.raises(RuntimeError, match="Not implemented on the CPU"):
             call()
 
