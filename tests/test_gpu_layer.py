@@ -330,6 +330,17 @@ def test_norm_offsets_beyond_32_bits():
         assert torch.equal(r[at], r2) and torch.equal(n[at], n2) and torch.equal(dx[at], d2)
 
 
+def test_norm_more_rows_than_a_grid_has_threads_for():
+    from instaorder_amd import residual_norm
+    rows = (1 << 26) + 7                              # a wave each: 2^32 threads and some
+    x = rand(gen(1), 1 << 20, 2, dtype=torch.bfloat16).repeat(65, 1)[:rows]
+    r, n = residual_norm(x, x, outer="layer")
+    first = residual_norm(x[:1 << 20], x[:1 << 20], outer="layer")
+    for i in range(0, rows, 1 << 20):
+        end = min(i + (1 << 20), rows)
+        assert torch.equal(r[i:end], first[0][:end - i]) and torch.equal(n[i:end], first[1][:end - i])
+
+
 # ---- orthogonalised update --------------------------------------------------------------------
 MUON = {torch.float32: 1e-4, torch.bfloat16: 2.0 ** -8 + 485 * 2.0 ** -17, torch.float16: 2.0 ** -11 + 485 * 2.0 ** -17}
 
