@@ -299,7 +299,7 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
     const bool need_x = needs(ctx, 0), need_y = needs(ctx, 1);
     if (need_x || (plain && need_y)) out[0] = at::empty(x.sizes(), options);
     if (need_y && !plain) out[1] = at::empty(x.sizes(), options);
-    if (needs(ctx, 2)) out[2] = at::empty(gate.sizes(), options);
+    if (needs(ctx, 2)) out[2] = rows ? at::empty(gate.sizes(), options) : at::zeros(gate.sizes(), options);   // a gate of no rows
     for (int i = 3; i < 8; ++i)
       if (needs(ctx, i)) out[i] = at::empty({width}, options);
     const size_t bytes = enc_residual_norm_backward_workspace_bytes(rows, width, group);

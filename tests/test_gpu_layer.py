@@ -266,6 +266,16 @@ def test_norm_shared_gates(lead):
     norm_check(norm_inputs(torch.float32, lead, 40, "rms", "rms", "sample", True, "w"), "rms", "rms")
 
 
+def test_norm_gradient_of_a_gate_without_rows():
+    from instaorder_amd import residual_norm
+    x, gate = rand(gen(1), 3, 0, 64), rand(gen(2), 3, 1, 64).requires_grad_(True)
+    junk = torch.full((3, 1, 64), 7.0, device="cuda")       # what the allocator hands out next
+    del junk
+    r, n = residual_norm(x, x, gate=gate, outer="rms")
+    grad, = torch.autograd.grad(r.sum() + n.sum(), gate)
+    assert torch.equal(grad, torch.zeros_like(gate))
+
+
 @pytest.mark.parametrize("grads", [("residual",), ("normed",)])
 def test_norm_one_gradient_only(grads):
     norm_check(norm_inputs(torch.float32, (4, 9), 72, "rms", "layer", "token", True, "wb"), "rms", "layer", grads=grads)
