@@ -29,7 +29,8 @@ def orthogonalize(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
 class Muon(torch.optim.Optimizer):
     """For parameters of two dimensions (others: another optimiser).  v = momentum * v + g;  u = g + momentum * v (nesterov)
     or v;  w <- w (1 - lr * weight_decay) - lr * sqrt(max(1, rows / cols)) * orthogonalize(u).  Matrices of one shape,
-    type and device are orthogonalised in one batch."""
+    type and device are orthogonalised in one batch.  v and u are fp32 whatever the type of w (in 16 bits a gradient below
+    2^-9 of v would leave it as it is); u is rounded to w's type for its orthogonalisation, whose result has that type."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS,
                  eps=1e-7):
@@ -42,6 +43,15 @@ class Muon(torch.optim.Optimizer):
                 if p.dim() != 2:
                     raise ValueError("Muon takes parameters of two dimensions, got one of shape %s" % (tuple(p.shape),))
 
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)           # casts to the parameters' types
+        new = [p for group in self.param_groups for p in group["params"]]
+        old = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for p, i in zip(new, old):
+            v = state_dict["state"].get(i, {}).get("momentum_buffer")
+            if v is not None:
+                self.state[p]["momentum_buffer"] = v.to(p.device, torch.float32, copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -53,13 +63,15 @@ class Muon(torch.optim.Optimizer):
             for p in group["params"]:
                 if p.grad is None:
                     continue
+                if p.grad.is_sparse:
+                    raise RuntimeError("Muon does not take sparse gradients")
                 state = self.state[p]
                 if "momentum_buffer" not in state:
-                    state["momentum_buffer"] = torch.zeros_like(p.grad)
+                    state["momentum_buffer"] = torch.zeros_like(p.grad, dtype=torch.float32)
                 v = state["momentum_buffer"]
                 v.mul_(group["momentum"]).add_(p.grad)
-                u = p.grad.add(v, alpha=group["momentum"]) if group["nesterov"] else v
-                alike.setdefault((p.shape, u.dtype, p.device), []).append((p, u))
+                u = p.grad.float().add(v, alpha=group["momentum"]) if group["nesterov"] else v
+                alike.setdefault((p.shape, p.dtype, p.device), []).append((p, u.to(p.dtype)))
             for (shape, _, _), members in alike.items():
                 batch = orthogonalize(torch.stack([u for _, u in members]), group["steps"], group["coefficients"],
                                       group["eps"])

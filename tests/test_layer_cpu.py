@@ -255,6 +255,35 @@ def test_muon_steps_are_the_rule():
         Muon([torch.nn.Parameter(torch.zeros(3, 3))], momentum=1.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_muon_keeps_its_momentum_in_fp32(dtype):
+    from instaorder_amd import Muon
+    g = torch.Generator().manual_seed(8)
+    grads = [(torch.randn(6, 4, generator=g) * s).to(dtype) for s in (1.0, 2e-3, 2e-3)]
+    runs = []
+    for reload in (False, True):
+        p = torch.nn.Parameter(torch.zeros(6, 4, dtype=dtype))
+        opt = Muon([p], lr=0.1, momentum=0.999)
+        for gr in grads:
+            p.grad = gr.clone()
+            opt.step()
+            if reload:
+                state = copy.deepcopy(opt.state_dict())
+                opt = Muon([p], lr=0.1, momentum=0.999)
+                opt.load_state_dict(state)
+        runs.append((p.detach(), opt.state[p]["momentum_buffer"]))
+    want = torch.zeros(6, 4, dtype=torch.float64)
+    for gr in grads:
+        want = 0.999 * want + gr.double()
+    for _, v in runs:
+        # two roundings a step to half of 2^-23 each, of values to 2 |v|
+        assert v.dtype == torch.float32 and float((v - want).abs().max()) <= 6 * 2.0 ** -24 * 2 * float(want.abs().max())
+    assert torch.equal(runs[0][0], runs[1][0])
+    p.grad = torch.eye(6, 4).to(dtype).to_sparse()
+    with pytest.raises(RuntimeError, match="sparse"):
+        opt.step()
+
+
 @pytest.mark.parametrize("activation", ["glu", "swiglu", "geglu", "reglu"])
 def test_encoder_layer_with_a_gated_block(activation):
     from instaorder_amd.encoder import GATED, MSDeformAttnTransformerEncoderLayer
