@@ -72,6 +72,7 @@ def build(force=False, verbose=False):
     finish(running)
     if bind:
         finish([start(link)])
+        os.remove(compile_[-2])
     return LIB
 
 
