@@ -43,7 +43,7 @@ uint32_t round8(uint32_t v) { return (v + 7u) & ~7u; }
 uint32_t ceil_div(size_t a, size_t b) { return (uint32_t)((a + b - 1) / b); }
 bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 bool known_type(int dtype) { return dtype == ENC_F32 || dtype == ENC_BF16 || dtype == ENC_F16; }
-int planes_of(int dtype) { return dtype == ENC_F32 ? 3 : 1; }
+int parts_of(int dtype) { return dtype == ENC_F32 ? 3 : 1; }
 
 // Hands out pieces of the caller's workspace; with base == nullptr it only counts.
 struct Carve {
