@@ -80,6 +80,16 @@ def test_feed_forward_big_tiles_and_slices(dtype):
     ffn_check(args, "silu", rand(gen(3), 4104, 248, dtype=dtype))
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("m, d, f, o", [(130, 72, 6000, 72), (700, 40, 3000, 40), (5, 1024, 4104, 520), (16, 2048, 2056, 2048),
+                                        (40, 520, 8192, 264), (300, 2048, 512, 1024), (520, 264, 4096, 1032)])
+def test_feed_forward_tiles_for_few_rows(dtype, m, d, f, o):
+    """Each tile that the number of rows and widths may choose, and products in many slices of k."""
+    args = ffn_inputs(dtype, m, d, f, o, True, seed=m)
+    ffn_check(args, "silu")
+    ffn_check(args, "gelu", rand(gen(4), m, o, dtype=dtype))
+
+
 @pytest.mark.parametrize("needs", [(True, False, False, False, False), (False, True, False, False, False),
                                    (False, False, True, False, True), (False, False, False, True, False),
                                    (False, False, False, False, True)])
@@ -376,6 +386,15 @@ def test_orthogonalize_sizes(dtype, rows, cols):
 @pytest.mark.parametrize("shape", [(1, 700, 1500), (1500, 600), (2, 1024, 1024), (20, 136, 200), (3, 260, 1000), (3, 1000, 260)])
 def test_orthogonalize_large_tiles_and_slices(dtype, shape):
     g = gen(5)
+    low = rand(g, *shape[:-1], 4) @ rand(g, *shape[:-2], 4, shape[-1])
+    muon_check((low + rand(g, *shape)).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("shape", [(8, 1000, 1000), (8, 1001, 997), (1300, 1700), (1700, 1300), (2049, 2300)])
+def test_orthogonalize_tiles(dtype, shape):
+    """Each tile of the symmetric products and of the updates, whole and in slices, with odd edges."""
+    g = gen(6)
     low = rand(g, *shape[:-1], 4) @ rand(g, *shape[:-2], 4, shape[-1])
     muon_check((low + rand(g, *shape)).to(dtype))
 
