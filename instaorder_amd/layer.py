@@ -19,8 +19,9 @@ def gated_feed_forward(x, w_in, b_in, w_out, b_out, activation="silu"):
     x [..., width]; w_in [2 * hidden, width] (value rows first, then gate rows -- the order of ``F.glu``); w_out
     [out_width, hidden]; biases may be None.  activation: "silu", "gelu" (by the error function), "sigmoid", "relu".
     fp32, bf16 or fp16, one type for all; sums are fp32, h is rounded to the type once.  Differentiable once in all five
-    tensors.  fp32 above 64 tokens and in the backward pass: an Inf among the inputs gives NaN (its parts multiply zeros), a
-    NaN stays one, and values below 2^-110 lose their low bits (their parts end at 2^-133)."""
+    tensors.  fp32 goes through three bf16 parts in the backward pass and in forward passes of many tokens: there an Inf among
+    the inputs gives NaN (its parts multiply zeros), a NaN stays one, and values below 2^-110 lose their low bits (their
+    parts end at 2^-133)."""
     bind = layer_ext._bind or layer_ext.bind()
     if x.is_cuda:
         return bind.gated_feed_forward(x, w_in, b_in, w_out, b_out, activation)
