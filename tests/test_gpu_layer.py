@@ -90,6 +90,24 @@ def test_feed_forward_tiles_for_few_rows(dtype, m, d, f, o):
     ffn_check(args, "gelu", rand(gen(4), m, o, dtype=dtype))
 
 
+@pytest.mark.parametrize("m, d, f, o", [(33, 2052, 4104, 36), (64, 2052, 4104, 37), (65, 36, 72, 7), (300, 100, 1032, 516), (1030, 68, 200, 64)])
+def test_feed_forward_fp32_in_place_and_not(m, d, f, o):
+    """Short fp32 forward passes read the tensors where they lie; the same call with rows that do not allow it."""
+    args = ffn_inputs(torch.float32, m, d, f, o, True, seed=m)
+    ffn_check(args, "silu")
+    ffn_check(args, "gelu", rand(gen(4), m, o))
+    wide = rand(gen(8), m, d + 5)
+    ffn_check([wide[:, 1:d + 1], *args[1:]], "silu")
+    shifted = torch.empty(2 * f * d + 1, device="cuda")[1:].view(2 * f, d)
+    ffn_check([args[0], shifted.copy_(args[1]), *args[2:]], "relu")
+    bad = args[0].clone()
+    bad[m // 2, d // 2] = float("nan")
+    from instaorder_amd import gated_feed_forward
+    y, clean = (gated_feed_forward(x, *args[1:]) for x in (bad, args[0]))
+    rest = torch.arange(m, device="cuda") != m // 2
+    assert torch.equal(y[rest], clean[rest]) and not y[m // 2].isfinite().any()
+
+
 @pytest.mark.parametrize("needs", [(True, False, False, False, False), (False, True, False, False, False),
                                    (False, False, True, False, True), (False, False, False, True, False),
                                    (False, False, False, False, True)])
