@@ -522,6 +522,42 @@ def test_side_stream_and_interleaved_calls():
         assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
+def test_two_threads_call_at_once():
+    """Forward and backward of two blocks from two threads, each on a stream of its own; an error in one is its own."""
+    import threading
+    from instaorder_amd import gated_feed_forward
+    cases = [block_inputs(torch.bfloat16, 2, 75, 64, 96, seed=s) for s in (1, 2)]
+
+    def work(t):
+        leaves = {k: v.detach().requires_grad_(True) for k, v in t.items()}
+        r, n = block(leaves)
+        return [r.detach(), n.detach(), *torch.autograd.grad(r.float().sum() + n.float().sum(), list(leaves.values()))]
+
+    want = [work(t) for t in cases]
+    torch.cuda.synchronize()
+    got, failed = [None, None], []
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                try:
+                    gated_feed_forward(cases[i]["x"], cases[i]["w_in"][:, 1:], None, cases[i]["w_out"], None)
+                except RuntimeError as e:
+                    failed.append(str(e))
+                got[i] = work(cases[i])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(failed) == 40 and all("w_in has shape" in f for f in failed)
+    for a, b in zip(got, want):
+        for x, y in zip(a, b):
+            assert torch.equal(x, y)
+
+
 @pytest.mark.parametrize("tokens", [1, 90])
 def test_captured_inference_replays_with_new_inputs(tokens):
     """Two graphs over the same operators, replayed in turn with eager calls between: no workspace is shared."""
