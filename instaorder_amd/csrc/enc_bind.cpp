@@ -2,9 +2,11 @@
 // allocation, torch's current stream and the autograd nodes, on top of the C ABI of libenc_hip.so (include/enc_hip.h).
 // Host code only.  A ctypes binding with Python autograd functions spent 170-200 us a forward and backward call, ten
 // times the kernels of a small block; this one holds the interpreter for the forward call alone.
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <string>
@@ -79,6 +81,14 @@ Tensor workspace(size_t bytes, const Tensor &x) {
 void done(const char *what, int rc) { TORCH_CHECK(rc == ENC_OK, what, ": ", enc_last_error()); }
 void on_gpu(const Tensor &x) { TORCH_CHECK(x.is_cuda(), "Not implemented on the CPU"); }
 
+// A trace records torch's own operators: of a call here it would keep the allocation of the result and lose the launch that
+// fills it.
+void not_traced(const char *what) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                  !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY),
+              what, ": cannot be traced (the trace would not hold the kernels)");
+}
+
 // Gradients that were formed by kernels: differentiating them again is an error, not zero.
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -126,6 +136,7 @@ FfnSizes check_ffn(const Tensor &x, const Tensor &w_in, const Tensor &b_in, cons
 
 Tensor ffn_forward(const Tensor &x, const Tensor &w_in, const Tensor &b_in, const Tensor &w_out, const Tensor &b_out, int act, Tensor *pre) {
   const char *what = "gated_feed_forward";
+  not_traced(what);
   const FfnSizes s = check_ffn(x, w_in, b_in, w_out, b_out);
   on_gpu(x);
   const c10::DeviceGuard guard(x.device());
@@ -158,6 +169,7 @@ struct GatedFeedForward : public torch::autograd::Function<GatedFeedForward> {
   }
   static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
     const char *what = "gated_feed_forward backward";
+    not_traced(what);
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &pre = saved[3], &grad = grads[0];
     const c10::DeviceGuard guard(x.device());
@@ -239,6 +251,7 @@ struct NormResults {
 };
 NormResults norm_forward(const NormInputs &t, int inner, int outer, double eps, bool want_residual, bool keep) {
   const char *what = "residual_norm";
+  not_traced(what);
   NormResults r;
   r.group = check_norm(t, inner, outer, want_residual);
   on_gpu(t.x);
@@ -277,6 +290,7 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
   }
   static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
     const char *what = "residual_norm backward";
+    not_traced(what);
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &y = saved[1], &gate = saved[2], &stats = saved[7];
     const int inner = (int)ctx->saved_data["inner"].toInt(), outer = (int)ctx->saved_data["outer"].toInt();
@@ -343,6 +357,7 @@ void check_orthogonalize(const Tensor &update, int64_t steps) {
 
 Tensor orthogonalize(const Tensor &given_update, int64_t steps, double a, double b, double c, double eps) {
   const char *what = "orthogonalize";
+  not_traced(what);
   check_orthogonalize(given_update, steps);
   on_gpu(given_update);
   const at::NoGradGuard no_grad;

@@ -4,7 +4,8 @@
     residual_norm(x, y, gate=, scale=, inner=, outer=, ...)
 
 GPU tensors always take the HIP kernels (errors propagate; the autograd nodes are in csrc/enc_bind.cpp); CPU tensors take
-an elementary PyTorch path by explicit device dispatch, as ``MSDeformAttn`` does."""
+an elementary PyTorch path by explicit device dispatch, as ``MSDeformAttn`` does.  On GPU tensors a call refuses to be traced
+(``torch.jit.trace``, ``make_fx``): the trace would hold the result's allocation and not the kernels."""
 import torch
 import torch.nn.functional as F
 

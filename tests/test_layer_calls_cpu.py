@@ -1,0 +1,27 @@
+"""CPU-only checks of how the layer operators are called: under tracing, forward-mode derivatives, autocast, hooks; with
+broadcast gates, after failed launches; and of the CPU paths beside the kernels."""
+import pytest
+import torch
+
+
+def raw_calls():
+    """The kernels' entry points by name, on CPU tensors: whatever they refuse they refuse before any device is touched."""
+    from instaorder_amd import layer_ext
+    b = layer_ext.bind()
+    w_in, w_out = torch.randn(12, 8), torch.randn(8, 6)
+    return {"gated_feed_forward": lambda x: b.gated_feed_forward(x, w_in, None, w_out, None, "silu"),
+            "residual_norm": lambda x: b.residual_norm(x, x, None, None, None, None, None, "layer", None, None, 1e-5, True)[1],
+            "orthogonalize": lambda x: b.orthogonalize(x, 5, 1.0, 1.0, 1.0, 1e-7)}
+
+
+@pytest.mark.parametrize("name", ["gated_feed_forward", "residual_norm", "orthogonalize"])
+def test_tracing_is_refused(name):
+    """A trace would hold the results' allocations and not the kernels that fill them."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, x = raw_calls()[name], torch.randn(4, 8)
+    with pytest.raises(RuntimeError, match=name + ".*cannot be traced"):
+        torch.jit.trace(call, x)
+    with pytest.raises(RuntimeError, match=name + ".*cannot be traced"):
+        make_fx(call)(x)
+    with pytest.raises(RuntimeError, match="Not implemented on the CPU"):       # and nothing is left behind
+        call(x)
