@@ -89,6 +89,12 @@ void not_traced(const char *what) {
               what, ": cannot be traced (the trace would not hold the kernels)");
 }
 
+// The kernels carry no tangents: a dual tensor's would be lost without a word.
+void no_tangents(const char *what, at::ArrayRef<Tensor> tensors) {
+  for (const Tensor &t : tensors)
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), what, ": forward-mode derivatives are not implemented");
+}
+
 // Gradients that were formed by kernels: differentiating them again is an error, not zero.
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -170,6 +176,7 @@ struct GatedFeedForward : public torch::autograd::Function<GatedFeedForward> {
   static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
     const char *what = "gated_feed_forward backward";
     not_traced(what);
+    no_tangents(what, grads);
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &pre = saved[3], &grad = grads[0];
     const c10::DeviceGuard guard(x.device());
@@ -205,6 +212,7 @@ Tensor gated_feed_forward(const Tensor &x, const Tensor &w_in, const MaybeTensor
                           const std::string &activation) {
   const int act = activation_code(activation);
   const Tensor bi = given(b_in), bo = given(b_out);
+  no_tangents("gated_feed_forward", {x, w_in, bi, w_out, bo});
   if (wants_grad({x, w_in, bi, w_out, bo})) return GatedFeedForward::apply(x, w_in, maybe(bi), w_out, maybe(bo), (int64_t)act);
   return ffn_forward(x, w_in, bi, w_out, bo, act, nullptr);
 }
@@ -291,6 +299,7 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
   static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
     const char *what = "residual_norm backward";
     not_traced(what);
+    no_tangents(what, grads);
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &y = saved[1], &gate = saved[2], &stats = saved[7];
     const int inner = (int)ctx->saved_data["inner"].toInt(), outer = (int)ctx->saved_data["outer"].toInt();
@@ -336,6 +345,7 @@ std::tuple<MaybeTensor, MaybeTensor> residual_norm(const Tensor &x, const Tensor
   const NormInputs t = {x, y, given(gate), given(scale), given(inner_weight), given(inner_bias), given(outer_weight), given(outer_bias)};
   const int in = norm_code(inner), out = norm_code(outer);
   Tensor residual, normed;
+  no_tangents("residual_norm", {t.x, t.y, t.gate, t.scale, t.iw, t.ib, t.ow, t.ob});
   if (wants_grad({t.x, t.y, t.gate, t.scale, t.iw, t.ib, t.ow, t.ob})) {
     const variable_list r = ResidualNorm::apply(t.x, t.y, maybe(t.gate), maybe(t.scale), maybe(t.iw), maybe(t.ib), maybe(t.ow), maybe(t.ob), (int64_t)in, (int64_t)out, eps, want_residual);
     if (want_residual) residual = r[0];
@@ -358,6 +368,7 @@ void check_orthogonalize(const Tensor &update, int64_t steps) {
 Tensor orthogonalize(const Tensor &given_update, int64_t steps, double a, double b, double c, double eps) {
   const char *what = "orthogonalize";
   not_traced(what);
+  no_tangents(what, {given_update});
   check_orthogonalize(given_update, steps);
   on_gpu(given_update);
   const at::NoGradGuard no_grad;

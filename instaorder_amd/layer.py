@@ -5,7 +5,8 @@
 
 GPU tensors always take the HIP kernels (errors propagate; the autograd nodes are in csrc/enc_bind.cpp); CPU tensors take
 an elementary PyTorch path by explicit device dispatch, as ``MSDeformAttn`` does.  On GPU tensors a call refuses to be traced
-(``torch.jit.trace``, ``make_fx``): the trace would hold the result's allocation and not the kernels."""
+(``torch.jit.trace``, ``make_fx``): the trace would hold the result's allocation and not the kernels; and it refuses dual
+tensors, whose tangents the kernels do not carry."""
 import torch
 import torch.nn.functional as F
 

@@ -25,3 +25,17 @@ def test_tracing_is_refused(name):
         make_fx(call)(x)
     with pytest.raises(RuntimeError, match="Not implemented on the CPU"):       # and nothing is left behind
         call(x)
+
+
+@pytest.mark.parametrize("name", ["gated_feed_forward", "residual_norm", "orthogonalize"])
+def test_forward_mode_derivatives_are_refused(name):
+    """With and without a graph to record: the kernels have no tangents, so none may be dropped."""
+    import torch.autograd.forward_ad as fwAD
+    call, x = raw_calls()[name], torch.randn(4, 8)
+    with fwAD.dual_level():
+        dual = fwAD.make_dual(x, torch.ones_like(x))
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), pytest.raises(RuntimeError, match=name + ".*forward-mode"):
+                call(dual)
+        with pytest.raises(RuntimeError, match="Not implemented on the CPU"):
+            call(x)
