@@ -239,10 +239,11 @@ int64_t check_norm(const NormInputs &t, int inner, int outer, bool want_residual
   TORCH_CHECK((inner != ENC_NORM_NONE || (!t.iw.defined() && !t.ib.defined())) && (outer != ENC_NORM_NONE || (!t.ow.defined() && !t.ob.defined())),
               what, ": a weight or bias of a norm that is None");
   if (!t.gate.defined()) return 1;
-  // x's shape, or ones in the last dimensions before the width: rows that share a gate
+  // x's shape, or ones in the last dimensions before the width: rows that share a gate (a dimension of x that is 1 itself
+  // among them adds none)
   size_t k = shape.size() - 1;
   if (t.gate.dim() == t.x.dim())
-    while (k && t.gate.size(k - 1) == 1 && shape[k - 1] != 1) --k;
+    while (k && t.gate.size(k - 1) == 1) --k;
   auto want = shape.vec();
   int64_t group = 1;
   for (size_t i = k; i + 1 < shape.size(); ++i) {

@@ -20,3 +20,32 @@ def test_a_gradient_with_a_tangent_is_refused():
             torch.autograd.grad(y, args[0], fwAD.make_dual(torch.ones_like(y), torch.ones_like(y)))
         dx, = torch.autograd.grad(call(), args[0], torch.ones_like(y))
         assert dx.isfinite().all()
+
+
+def gradients(t, inner, outer):
+    """Results and all gradients of a residual norm of the leaves `t`; none may be missing."""
+    from instaorder_amd import residual_norm
+    leaves = {k: v.detach().requires_grad_(True) for k, v in t.items()}
+    r, n = residual_norm(**leaves, inner=inner, outer=outer)
+    g = gen(99)
+    grads = {"residual": rand(g, *t["x"].shape, dtype=t["x"].dtype), "normed": rand(g, *t["x"].shape, dtype=t["x"].dtype)}
+    got = torch.autograd.grad([r, n], list(leaves.values()), list(grads.values()))
+    return {"residual": r.detach(), "normed": n.detach(), **{"d_" + k: v for k, v in zip(leaves, got)}}, grads
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("lead, gate", [((3, 1), (1, 1)), ((2, 3, 1), (2, 1, 1)), ((3, 1, 5), (1, 1, 1)), ((3, 1, 5), (3, 1, 1)),
+                                        ((700, 1), (1, 1)), ((1, 1), (1, 1))])
+def test_gates_shared_over_dimensions_of_one(dtype, lead, gate):
+    t = norm_inputs(dtype, lead, 72, "layer", "rms", None, True, "wb")
+    t["gate"] = rand(gen(3), *gate, 72, dtype=dtype)
+    got, grads = gradients(t, "layer", "rms")
+    want = R.residual_norm(t, "layer", "rms", 1e-5, grads)
+    assert set(got) == set(want)
+    rows = t["x"].numel() // 72
+    for k, v in got.items():
+        # a row's sums are at most 16 + 6 + 16 steps of 32 bits, a column's 64 + 4 sqrt(rows); 16 for the spread of the inputs
+        w = want[k]
+        size, steps = (w.abs().amax(-1, keepdim=True), 64) if v.shape == t["x"].shape else (w.abs().max(), 64 + 4 * rows ** 0.5)
+        assert v.shape == w.shape and v.dtype == dtype
+        R.within(v, w, (R.U[dtype] * w.abs()).clamp(min=R.FLOOR[dtype]) + steps * 16 * R.U32 * (size + 1.0) + R.TINY, k)

@@ -39,3 +39,28 @@ def test_forward_mode_derivatives_are_refused(name):
                 call(dual)
         with pytest.raises(RuntimeError, match="Not implemented on the CPU"):
             call(x)
+
+
+GATES = [((3, 1), (1, 1)), ((8, 5), (1, 1)), ((3, 1), (3, 1)), ((2, 3, 1), (2, 1, 1)), ((2, 3, 1), (1, 1, 1)),
+         ((3, 1, 5), (1, 1, 1)), ((3, 1, 5), (3, 1, 1)), ((1, 1), (1, 1)), ((4, 1, 1), (1, 1, 1)), ((0, 1), (1, 1)),
+         ((2, 1, 0), (2, 1, 1))]
+
+
+@pytest.mark.parametrize("lead, gate", GATES)
+def test_gates_shared_over_dimensions_of_one(lead, gate):
+    """One token of a batch: x [batch, 1, width] under a gate [1, 1, width]."""
+    from instaorder_amd import residual_norm
+    g = torch.Generator().manual_seed(1)
+    x, y, v = (torch.randn(*s, 16, generator=g) for s in (lead, lead, gate))
+    r, _ = residual_norm(x, y, gate=v, outer="rms")
+    assert torch.equal(r, x + y * v)
+    with pytest.raises(RuntimeError, match="gate has shape"):
+        residual_norm(x, y, gate=torch.zeros(*[2 if n == 1 else n for n in gate], 16), outer="rms")
+
+
+def test_gates_in_other_dimensions_are_refused():
+    from instaorder_amd import residual_norm
+    x = torch.zeros(3, 4, 5, 16)
+    for gate in ((3, 1, 5, 16), (1, 4, 1, 16), (1, 4, 5, 16), (4, 5, 16), (5, 16), (3, 4, 5, 1), (16,)):
+        with pytest.raises(RuntimeError, match="gate has shape"):
+            residual_norm(x, x, gate=torch.zeros(gate))
