@@ -8,6 +8,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <tuple>
 #include <type_traits>
 
 #include "enc_hip.h"
@@ -22,17 +23,25 @@ namespace {
 // ---------------------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------------------
-// An error some other library left pending on this thread is neither reported as ours nor consumed: a launch has
-// failed when the pending error afterwards is a different one.
+// A launch has failed if the runtime says so of that launch.  (The thread's pending error does not tell: one that some other
+// library left there, or an earlier failure of the same kind, would hide it.)  Our own failure is reported and does not
+// stay pending; an error that was there before a call that succeeds is left alone.
 struct Call {
   const char *who;
   hipStream_t st;
-  hipError_t pending;
-  Call(const char *w, void *stream) : who(w), st(static_cast<hipStream_t>(stream)), pending(hipPeekAtLastError()) {}
-  int launched() const {
-    const hipError_t e = hipPeekAtLastError();
-    if (e != hipSuccess && e != pending)
+  Call(const char *w, void *stream) : who(w), st(static_cast<hipStream_t>(stream)) {}
+  template <typename... P, typename... A>
+  int launch(void (*kernel)(P...), dim3 blocks, dim3 threads, A... args) const {
+    static_assert(sizeof...(P) == sizeof...(A), "the kernel's arguments");
+    std::tuple<P...> values(static_cast<P>(args)...);
+    void *pointers[sizeof...(P)];
+    int at = 0;
+    std::apply([&](auto &...v) { ((pointers[at++] = &v), ...); }, values);
+    const hipError_t e = hipLaunchKernel(reinterpret_cast<const void *>(kernel), blocks, threads, pointers, 0, st);
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
       return fail(ENC_ERR_LAUNCH, "%s: kernel launch failed: %s", who, hipGetErrorString(e));
+    }
     g_launches.fetch_add(1, std::memory_order_relaxed);
     return ENC_OK;
   }

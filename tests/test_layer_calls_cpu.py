@@ -64,3 +64,18 @@ def test_gates_in_other_dimensions_are_refused():
     for gate in ((3, 1, 5, 16), (1, 4, 1, 16), (1, 4, 5, 16), (4, 5, 16), (5, 16), (3, 4, 5, 1), (16,)):
         with pytest.raises(RuntimeError, match="gate has shape"):
             residual_norm(x, x, gate=torch.zeros(gate))
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the launches have to fail: the pointers are made up")
+def test_every_failed_launch_is_reported():
+    """Without a device each launch fails alike: the second failure is one too, and neither is counted or left pending."""
+    from test_layer_cpu import lib, norm_call
+    handle = lib()
+    before = handle.enc_launch_count()
+    for _ in range(3):
+        assert norm_call() == 2
+        assert "kernel launch failed" in handle.enc_last_error().decode()
+        assert handle.enc_orthogonalize(0, 256, 256, 1, 8, 8, 5, 1.0, 1.0, 1.0, 1e-7, 256, 1 << 30, None) == 2
+        assert handle.enc_gated_ffn_forward(1, 0, 16, 32, 16, None, 16, None, 4, 32, 8, 32, 16, None, 256, 1 << 30, None) == 2
+        assert handle.enc_gated_ffn_backward(1, 0, 16, 32, 16, 16, 16, 16, 32, 4, 32, 8, 32, 16, 16, 16, 16, 16, 256, 1 << 30, None) == 2
+    assert handle.enc_launch_count() == before
