@@ -15,6 +15,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <tuple>
 
 #include "msda_hip.h"
 
@@ -28,14 +29,27 @@ namespace {
 // ---------------------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------------------
-// hipGetLastError is per thread and sticky until read.  An error some other library left pending on this thread
-// must neither be reported as a failed MSDA launch nor be consumed here (the application's own check would never
-// see it): every entry point notes what is pending when it is entered (check_dims), and a launch has failed when
-// the pending error afterwards is a different one.  Nothing here resets the thread's error state.
-thread_local hipError_t g_pending = hipSuccess;
+// A launch has failed if the runtime says so of that launch.  (hipGetLastError is per thread and sticky until read: an error
+// that some other library left pending there, or an earlier failure of the same kind, would hide it.)  Our own failure is
+// reported and does not stay pending; an error that was there before a call that succeeds is neither reported nor
+// consumed (the application's own check would never see it).
+thread_local hipError_t g_launch = hipSuccess;
+
+template <typename... P, typename... A>
+void launch(void (*kernel)(P...), dim3 blocks, dim3 threads, size_t lds, hipStream_t st, A... args) {
+  static_assert(sizeof...(P) == sizeof...(A), "the kernel's arguments");
+  std::tuple<P...> values(static_cast<P>(args)...);
+  void *pointers[sizeof...(P)];
+  int at = 0;
+  std::apply([&](auto &...v) { ((pointers[at++] = &v), ...); }, values);
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void *>(kernel), blocks, threads, pointers, lds, st);
+  if (e == hipSuccess) return;
+  (void)hipGetLastError();
+  g_launch = e;
+}
 
 int check_dims(const char *who, int N, int S, int M, int D, int L, int Lq, int P) {
-  g_pending = hipPeekAtLastError();
+  g_launch = hipSuccess;
   if (N < 0 || S < 0 || M <= 0 || D <= 0 || L <= 0 || Lq < 0 || P <= 0)
     return fail(MSDA_ERR_INVALID_ARGUMENT,
                 "%s: bad dimensions batch=%d spatial_size=%d num_heads=%d channels=%d "
@@ -45,9 +59,9 @@ int check_dims(const char *who, int N, int S, int M, int D, int L, int Lq, int P
 }
 
 int check_launch(const char *who) {
-  const hipError_t e = hipPeekAtLastError();
-  if (e != hipSuccess && e != g_pending)
-    return fail(MSDA_ERR_LAUNCH, "%s: kernel launch failed: %s", who, hipGetErrorString(e));
+  const hipError_t e = g_launch;
+  g_launch = hipSuccess;
+  if (e != hipSuccess) return fail(MSDA_ERR_LAUNCH, "%s: kernel launch failed: %s", who, hipGetErrorString(e));
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return MSDA_OK;
 }
@@ -78,8 +92,8 @@ int forward_generic(const T *value, const int64_t *shapes, const int64_t *lsi, c
     return fail(MSDA_ERR_INVALID_ARGUMENT, "msda_forward: problem too large (%zu blocks)", nblk);
 #define MSDA_LAUNCH_FWD(GG)                                                                  \
   case GG:                                                                                   \
-    hipLaunchKernelGGL((msda_fwd_generic_kernel<T, GG>), dim3((unsigned)nblk), dim3(256), 0, \
-                       st, value, shapes, lsi, loc, aw, S, M, D, L, Lq, P, npairs, out);     \
+    launch((msda_fwd_generic_kernel<T, GG>), dim3((unsigned)nblk), dim3(256), 0, \
+           st, value, shapes, lsi, loc, aw, S, M, D, L, Lq, P, npairs, out);                 \
     break;
   switch (G) {
     MSDA_LAUNCH_FWD(1)
@@ -105,9 +119,9 @@ int backward_generic(const T *value, const int64_t *shapes, const int64_t *lsi, 
     return fail(MSDA_ERR_INVALID_ARGUMENT, "msda_backward: problem too large (%zu blocks)", nblk);
 #define MSDA_LAUNCH_BWD(GG)                                                                  \
   case GG:                                                                                   \
-    hipLaunchKernelGGL((msda_bwd_generic_kernel<T, GG>), dim3((unsigned)nblk), dim3(256), 0, \
-                       st, grad_out, value, shapes, lsi, loc, aw, S, M, D, L, Lq, P, npairs, \
-                       grad_value, grad_loc, grad_aw);                                       \
+    launch((msda_bwd_generic_kernel<T, GG>), dim3((unsigned)nblk), dim3(256), 0, \
+           st, grad_out, value, shapes, lsi, loc, aw, S, M, D, L, Lq, P, npairs,             \
+           grad_value, grad_loc, grad_aw);                                                   \
     break;
   switch (G) {
     MSDA_LAUNCH_BWD(1)
@@ -167,20 +181,20 @@ void launch_forward_d32(const VT *value, const int64_t *shapes, const int64_t *l
       aligned16(out)) {
     const uint32_t nq = (uint32_t)(npairs / (size_t)M), nunits = ((nq + GP - 1u) / GP) * (uint32_t)M;
     const uint32_t nblk = (nunits + 3u) / 4u;
-    hipLaunchKernelGGL((msda_fwd_d32_qh_kernel<VT, false>), dim3(nblk), dim3(256), lds, st, value, shapes, lsi,
-                       loc, aw, (const float *)nullptr, S, M, L, Lq, P, nq, nunits, nblk,
-                       aligned16(loc) && (reinterpret_cast<uintptr_t>(aw) & 7u) == 0, fwd_div_magic((uint32_t)(L * P)),
-                       fwd_div_magic((uint32_t)P), fwd_div_magic32((uint32_t)M, nunits), fwd_div_magic_lq((uint32_t)Lq, nq, GP),
-                       fwd_region_log2(), out);
+    launch((msda_fwd_d32_qh_kernel<VT, false>), dim3(nblk), dim3(256), lds, st, value, shapes, lsi,
+           loc, aw, (const float *)nullptr, S, M, L, Lq, P, nq, nunits, nblk,
+           aligned16(loc) && (reinterpret_cast<uintptr_t>(aw) & 7u) == 0, fwd_div_magic((uint32_t)(L * P)),
+           fwd_div_magic((uint32_t)P), fwd_div_magic32((uint32_t)M, nunits), fwd_div_magic_lq((uint32_t)Lq, nq, GP),
+           fwd_region_log2(), out);
     return;
   }
   const uint32_t nblk = (uint32_t)((npairs + 31) / 32);
   if (P == 4 && aligned16(loc) && aligned16(aw))
-    hipLaunchKernelGGL((msda_fwd_d32_kernel<VT, true>), dim3(nblk), dim3(256), 0, st, value, shapes,
-                       lsi, loc, aw, S, M, L, Lq, P, (uint32_t)npairs, nblk, out);
+    launch((msda_fwd_d32_kernel<VT, true>), dim3(nblk), dim3(256), 0, st, value, shapes,
+           lsi, loc, aw, S, M, L, Lq, P, (uint32_t)npairs, nblk, out);
   else
-    hipLaunchKernelGGL((msda_fwd_d32_kernel<VT, false>), dim3(nblk), dim3(256), 0, st, value, shapes,
-                       lsi, loc, aw, S, M, L, Lq, P, (uint32_t)npairs, nblk, out);
+    launch((msda_fwd_d32_kernel<VT, false>), dim3(nblk), dim3(256), 0, st, value, shapes,
+           lsi, loc, aw, S, M, L, Lq, P, (uint32_t)npairs, nblk, out);
 }
 
 template <>
@@ -383,20 +397,20 @@ int launch_binned_group(const char *who, const VT *value, const int64_t *shapes,
   const uint32_t spi = (uint32_t)((size_t)Lq * M * L);          // quads per image
   const uint32_t bpi = (spi + binned::BIN_QB - 1) / binned::BIN_QB;
   const int cus = num_cus();
-  hipLaunchKernelGGL(binned::msda_bwd_bin_zero_kernel, dim3(cus), dim3(256), 0, st, shapes, lsi, N, S, M, L,
-                     Lq, P, key_cap, GV16 ? 3u : 4u, counts, static_cast<void *>(grad_value), grad_loc, grad_aw);
+  launch(binned::msda_bwd_bin_zero_kernel, dim3(cus), dim3(256), 0, st, shapes, lsi, N, S, M, L,
+         Lq, P, key_cap, GV16 ? 3u : 4u, counts, static_cast<void *>(grad_value), grad_loc, grad_aw);
   if (int rc = check_launch(who)) return rc;
   const uint64_t magic_ml = (((uint64_t)1 << 40) + (uint64_t)(M * L) - 1) / (uint64_t)(M * L);
   const uint64_t magic_l = (((uint64_t)1 << 40) + (uint64_t)L - 1) / (uint64_t)L;
   const uint32_t kcap = binned_kcap(S, M, L);
   // the fused boundary: grad_loc / grad_aw in the scratch layout [M, L, N * Lq, P] (binned.inc, PLANAR)
   const uint32_t planar_nq = planar ? (uint32_t)((size_t)N * Lq) : 0u;
-  hipLaunchKernelGGL(binned::msda_bwd_bin_kernel<0>, dim3((uint32_t)N * bpi), dim3(binned::BIN_NT),
-                     kcap * 4, st, shapes, lsi, loc, N, S, M, L, Lq, P, spi, bpi, magic_ml, magic_l, key_cap, 0u, kcap,
-                     planar_nq, counts, desc, entries, grad_loc, grad_aw);
+  launch(binned::msda_bwd_bin_kernel<0>, dim3((uint32_t)N * bpi), dim3(binned::BIN_NT),
+         kcap * 4, st, shapes, lsi, loc, N, S, M, L, Lq, P, spi, bpi, magic_ml, magic_l, key_cap, 0u, kcap,
+         planar_nq, counts, desc, entries, grad_loc, grad_aw);
   if (int rc = check_launch(who)) return rc;
-  hipLaunchKernelGGL(binned::msda_bwd_bin_scan_kernel, dim3(1), dim3(1024), 0, st, shapes, lsi, N, S, M, L,
-                     key_cap, (uint32_t)reg.e_cap, reg.rounds, counts, offs);
+  launch(binned::msda_bwd_bin_scan_kernel, dim3(1), dim3(1024), 0, st, shapes, lsi, N, S, M, L,
+         key_cap, (uint32_t)reg.e_cap, reg.rounds, counts, offs);
   if (int rc = check_launch(who)) return rc;
   const size_t gv_elems = (size_t)N * S * M * 32;
   float *sums = nullptr;                               // split mode: what the parts of a tile's list add into
@@ -411,40 +425,40 @@ int launch_binned_group(const char *who, const VT *value, const int64_t *shapes,
   // without lists returns at once
   for (int r = 0; r < reg.rounds; ++r) {
     if (reg.rounds == 1)
-      hipLaunchKernelGGL(binned::msda_bwd_bin_kernel<1>, dim3((uint32_t)N * bpi), dim3(binned::BIN_NT),
-                         kcap * 4, st, shapes, lsi, loc, N, S, M, L, Lq, P, spi, bpi, magic_ml, magic_l, key_cap, 0u,
-                         kcap, planar_nq, counts, desc, entries, grad_loc, grad_aw);
+      launch(binned::msda_bwd_bin_kernel<1>, dim3((uint32_t)N * bpi), dim3(binned::BIN_NT),
+             kcap * 4, st, shapes, lsi, loc, N, S, M, L, Lq, P, spi, bpi, magic_ml, magic_l, key_cap, 0u,
+             kcap, planar_nq, counts, desc, entries, grad_loc, grad_aw);
     else
-      hipLaunchKernelGGL(binned::msda_bwd_bin_kernel<2>, dim3((uint32_t)N * bpi), dim3(binned::BIN_NT),
-                         kcap * 4, st, shapes, lsi, loc, N, S, M, L, Lq, P, spi, bpi, magic_ml, magic_l, key_cap,
-                         (uint32_t)r, kcap, planar_nq, counts, desc, entries, grad_loc, grad_aw);
+      launch(binned::msda_bwd_bin_kernel<2>, dim3((uint32_t)N * bpi), dim3(binned::BIN_NT),
+             kcap * 4, st, shapes, lsi, loc, N, S, M, L, Lq, P, spi, bpi, magic_ml, magic_l, key_cap,
+             (uint32_t)r, kcap, planar_nq, counts, desc, entries, grad_loc, grad_aw);
     if (int rc = check_launch(who)) return rc;
     uint32_t *work = ctrl + binned::CTRL_WORK + r;
     if constexpr (!GV16) {
       if (planar) {                                      // (fp32 grad_value only: the fused boundary's)
-        hipLaunchKernelGGL((binned::msda_bwd_binned_kernel<VT, float, true>), dim3(2 * cus), dim3(binned::NT), 0, st,
-                           grad_out, value, shapes, lsi, loc, aw, offs, entries, zero_word, work, ctrl + r,
-                           key_cap, N, S, M, L, P, split ? 1 : 0, planar_nq, reinterpret_cast<float *>(grad_value),
-                           split ? sums : (float *)nullptr, grad_loc, grad_aw);
+        launch((binned::msda_bwd_binned_kernel<VT, float, true>), dim3(2 * cus), dim3(binned::NT), 0, st,
+               grad_out, value, shapes, lsi, loc, aw, offs, entries, zero_word, work, ctrl + r,
+               key_cap, N, S, M, L, P, split ? 1 : 0, planar_nq, reinterpret_cast<float *>(grad_value),
+               split ? sums : (float *)nullptr, grad_loc, grad_aw);
         if (int rc = check_launch(who)) return rc;
         continue;
       }
     }
     if (split)
       // every tile of this group adds to, or stores into, the zero-filled fp32 tensor
-      hipLaunchKernelGGL((binned::msda_bwd_binned_kernel<VT, float>), dim3(2 * cus), dim3(binned::NT), 0, st,
-                         grad_out, value, shapes, lsi, loc, aw, offs, entries, zero_word, work, ctrl + r,
-                         key_cap, N, S, M, L, P, 1, 0u, sums, sums, grad_loc, grad_aw);
+      launch((binned::msda_bwd_binned_kernel<VT, float>), dim3(2 * cus), dim3(binned::NT), 0, st,
+             grad_out, value, shapes, lsi, loc, aw, offs, entries, zero_word, work, ctrl + r,
+             key_cap, N, S, M, L, P, 1, 0u, sums, sums, grad_loc, grad_aw);
     else
-      hipLaunchKernelGGL((binned::msda_bwd_binned_kernel<VT, GT>), dim3(2 * cus), dim3(binned::NT), 0, st,
-                         grad_out, value, shapes, lsi, loc, aw, offs, entries, zero_word, work, ctrl + r,
-                         key_cap, N, S, M, L, P, 0, 0u, grad_value, (float *)nullptr, grad_loc, grad_aw);
+      launch((binned::msda_bwd_binned_kernel<VT, GT>), dim3(2 * cus), dim3(binned::NT), 0, st,
+             grad_out, value, shapes, lsi, loc, aw, offs, entries, zero_word, work, ctrl + r,
+             key_cap, N, S, M, L, P, 0, 0u, grad_value, (float *)nullptr, grad_loc, grad_aw);
     if (int rc = check_launch(who)) return rc;
   }
   if (split && GV16) {
-    hipLaunchKernelGGL(binned::msda_bwd_round_kernel, dim3(2 * cus), dim3(256), 0, st, sums,
-                       reinterpret_cast<bf16_t *>(grad_value), shapes, lsi, N, S, M, L, key_cap,
-                       (uint64_t)(gv_elems / 4));
+    launch(binned::msda_bwd_round_kernel, dim3(2 * cus), dim3(256), 0, st, sums,
+           reinterpret_cast<bf16_t *>(grad_value), shapes, lsi, N, S, M, L, key_cap,
+           (uint64_t)(gv_elems / 4));
     return check_launch(who);
   }
   return MSDA_OK;
@@ -637,10 +651,10 @@ int fused_forward(const char *who, const VT *value, const int64_t *shapes, const
   const size_t lds = (size_t)4 * ((size_t)2 * GP * (size_t)(L * P + 1) * 16 + (((size_t)GP * L * P + 3) / 4) * 16);
   const uint32_t nq = (uint32_t)((size_t)N * Lq), nunits = ((nq + GP - 1u) / GP) * (uint32_t)M;
   const uint32_t nblk = (nunits + 3u) / 4u;
-  hipLaunchKernelGGL((msda_fwd_d32_qh_kernel<VT, true>), dim3(nblk), dim3(256), lds,
-                     static_cast<hipStream_t>(stream), value, shapes, lsi, off, logits, refp, S, M, L, Lq, P,
-                     nq, nunits, nblk, false, fwd_div_magic((uint32_t)(L * P)), fwd_div_magic((uint32_t)P),
-                     fwd_div_magic32((uint32_t)M, nunits), fwd_div_magic_lq((uint32_t)Lq, nq, GP), fwd_region_log2(), out);
+  launch((msda_fwd_d32_qh_kernel<VT, true>), dim3(nblk), dim3(256), lds,
+         static_cast<hipStream_t>(stream), value, shapes, lsi, off, logits, refp, S, M, L, Lq, P,
+         nq, nunits, nblk, false, fwd_div_magic((uint32_t)(L * P)), fwd_div_magic((uint32_t)P),
+         fwd_div_magic32((uint32_t)M, nunits), fwd_div_magic_lq((uint32_t)Lq, nq, GP), fwd_region_log2(), out);
   return check_launch(who);
 }
 
@@ -686,8 +700,8 @@ int fused_backward(const char *who, bool bf16, const void *value, const int64_t 
   if (L * P > FUSED_MAX_LP)
     return fail(MSDA_ERR_INVALID_ARGUMENT, "%s: num_levels * num_point must be <= %d", who, FUSED_MAX_LP);
   if (npairs) {
-    hipLaunchKernelGGL(msda_fused_prologue_kernel, dim3((unsigned)nblk), dim3(256), 0, st, shapes, refp, off,
-                       logits, M, L, P, npairs, loc, aw);
+    launch(msda_fused_prologue_kernel, dim3((unsigned)nblk), dim3(256), 0, st, shapes, refp, off,
+           logits, M, L, P, npairs, loc, aw);
     if (int rc = check_launch(who)) return rc;
   }
   int rc;
@@ -709,12 +723,12 @@ int fused_backward(const char *who, bool bf16, const void *value, const int64_t 
   if (npairs && planar) {
     const uint32_t NQ = (uint32_t)((size_t)N * Lq), qb = (uint32_t)(FUSED_PB / M > 0 ? FUSED_PB / M : 1);
     const size_t lds = (size_t)qb * M * L * P * 3 * sizeof(float);
-    hipLaunchKernelGGL(msda_fused_epilogue_planar_kernel, dim3((NQ + qb - 1) / qb), dim3(256), lds, st, shapes, aw, M, L,
-                       P, NQ, qb, gl_scratch, ga_scratch, grad_off, grad_logits);
+    launch(msda_fused_epilogue_planar_kernel, dim3((NQ + qb - 1) / qb), dim3(256), lds, st, shapes, aw, M, L,
+           P, NQ, qb, gl_scratch, ga_scratch, grad_off, grad_logits);
     if (int rc2 = check_launch(who)) return rc2;
   } else if (npairs) {
-    hipLaunchKernelGGL(msda_fused_epilogue_kernel, dim3((unsigned)nblk), dim3(256), 0, st, shapes, aw, L, P,
-                       npairs, grad_off, grad_logits);
+    launch(msda_fused_epilogue_kernel, dim3((unsigned)nblk), dim3(256), 0, st, shapes, aw, L, P,
+           npairs, grad_off, grad_logits);
     if (int rc2 = check_launch(who)) return rc2;
   }
   return MSDA_OK;

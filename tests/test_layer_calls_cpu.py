@@ -79,3 +79,18 @@ def test_every_failed_launch_is_reported():
         assert handle.enc_gated_ffn_forward(1, 0, 16, 32, 16, None, 16, None, 4, 32, 8, 32, 16, None, 256, 1 << 30, None) == 2
         assert handle.enc_gated_ffn_backward(1, 0, 16, 32, 16, 16, 16, 16, 32, 4, 32, 8, 32, 16, 16, 16, 16, 16, 256, 1 << 30, None) == 2
     assert handle.enc_launch_count() == before
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the launches have to fail: the pointers are made up")
+def test_every_failed_launch_of_the_attention_op_is_reported():
+    import ctypes
+    import os
+    from conftest import ROOT
+    handle = ctypes.CDLL(os.path.join(ROOT, "instaorder_amd", "libmsda_hip.so"))
+    handle.msda_last_error.restype, handle.msda_launch_count.restype = ctypes.c_char_p, ctypes.c_uint64
+    before, made_up = handle.msda_launch_count(), [ctypes.c_void_p(256)] * 5
+    for _ in range(3):
+        for head in (32, 24):                           # the kernels for 32 channels a head, and those for any
+            assert handle.msda_forward_f32(*made_up, 1, 6, 2, head, 1, 4, 2, ctypes.c_void_p(256), None) == 2
+            assert b"kernel launch failed" in handle.msda_last_error()
+    assert handle.msda_launch_count() == before
