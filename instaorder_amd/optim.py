@@ -19,7 +19,8 @@ def orthogonalize(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     x = update.float()
     tall = x.shape[-2] > x.shape[-1]
     x = x.mT if tall else x
-    x = x / x.square().sum((-2, -1), keepdim=True).sqrt().clamp(min=eps)
+    norm = x.double().square().sum((-2, -1), keepdim=True).sqrt()        # squares of 32-bit values leave 32 bits
+    x = (x / norm.clamp(min=eps)).float()
     for _ in range(steps):
         gram = x @ x.mT
         x = a * x + (b * gram + c * (gram @ gram)) @ x

@@ -94,3 +94,11 @@ def test_every_failed_launch_of_the_attention_op_is_reported():
             assert handle.msda_forward_f32(*made_up, 1, 6, 2, head, 1, 4, 2, ctypes.c_void_p(256), None) == 2
             assert b"kernel launch failed" in handle.msda_last_error()
     assert handle.msda_launch_count() == before
+
+
+@pytest.mark.parametrize("factor", [2.0 ** -60, 2.0 ** 100])
+def test_cpu_orthogonalize_of_values_whose_squares_leave_32_bits(factor):
+    from instaorder_amd import orthogonalize
+    u = torch.randn(2, 6, 9, generator=torch.Generator().manual_seed(2))
+    want = orthogonalize(u)
+    assert torch.allclose(orthogonalize(u * factor, eps=1e-30), want, rtol=1e-5, atol=1e-6)
