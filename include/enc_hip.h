@@ -30,6 +30,8 @@ extern "C" {
 #define ENC_F32 0
 #define ENC_BF16 1
 #define ENC_F16 2
+/* enc_orthogonalize and its workspace query: | ENC_BF16 or ENC_F16, the result's type, of an update in fp32 */
+#define ENC_UPDATE_F32 16
 
 #define ENC_ACT_SILU 0
 #define ENC_ACT_GELU 1 /* x * Phi(x), by the error function */
@@ -101,7 +103,8 @@ int enc_residual_norm_backward(int dtype, int inner, int outer, const void *x, i
  * Orthogonalised update (Newton-Schulz steps of the Muon optimiser), a batch of contiguous matrices [batch, rows, cols]:
  *   X = update / max(|update|, eps)   (Frobenius norm, summed in 64 bits)
  *   `steps` times:  A = X X^T;  X = a X + (b A + c A A) X      (on the short side: A = X^T X and X from the left if rows > cols)
- * out: X in `dtype`; it may be `update` itself.  Iterates keep 24 bits (ENC_F32) or 16 (the 16-bit types).
+ * out: X in `dtype`; it may be `update` itself.  Iterates keep 24 bits (ENC_F32) or 16 (the 16-bit types).  With
+ * ENC_UPDATE_F32 the update is fp32 and only the result has 16 bits: values that the type does not reach keep their direction.
  * Limits: steps 1 to 100, batch < 65536, the short side at most 65536.
  */
 size_t enc_orthogonalize_workspace_bytes(int dtype, int64_t batch, int64_t rows, int64_t cols);

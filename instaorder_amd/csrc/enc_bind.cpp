@@ -359,25 +359,32 @@ std::tuple<MaybeTensor, MaybeTensor> residual_norm(const Tensor &x, const Tensor
 }
 
 // ---- orthogonalised update --------------------------------------------------------------------
-void check_orthogonalize(const Tensor &update, int64_t steps) {
+typedef std::optional<at::ScalarType> MaybeType;
+// The C entry's type: the result's, the update's own if none is given; of an fp32 update also a 16-bit one.
+int check_orthogonalize(const Tensor &update, int64_t steps, MaybeType type) {
   const char *what = "orthogonalize";
-  dtype_code(what, update);
+  int code = dtype_code(what, update);
+  if (type && *type != update.scalar_type()) {
+    TORCH_CHECK(code == ENC_F32 && (*type == at::kBFloat16 || *type == at::kHalf), what, ": a result of ", *type, " is not made of an update of ",
+                update.scalar_type());
+    code = (*type == at::kHalf ? ENC_F16 : ENC_BF16) | ENC_UPDATE_F32;
+  }
   TORCH_CHECK(update.dim() >= 2 && update.size(-1) >= 1 && update.size(-2) >= 1, what, ": update must be [..., rows, cols] with at least one of each");
   TORCH_CHECK(steps >= 1 && steps <= 100, what, ": steps must be 1 to 100");
+  return code;
 }
 
-Tensor orthogonalize(const Tensor &given_update, int64_t steps, double a, double b, double c, double eps) {
+Tensor orthogonalize(const Tensor &given_update, int64_t steps, double a, double b, double c, double eps, MaybeType type) {
   const char *what = "orthogonalize";
   not_traced(what);
   no_tangents(what, {given_update});
-  check_orthogonalize(given_update, steps);
+  const int code = check_orthogonalize(given_update, steps, type);
   on_gpu(given_update);
   const at::NoGradGuard no_grad;
   const c10::DeviceGuard guard(given_update.device());
   const Tensor update = given_update.contiguous();
-  const Tensor out = at::empty(update.sizes(), update.options().requires_grad(false));
+  const Tensor out = at::empty(update.sizes(), update.options().dtype(type ? *type : update.scalar_type()).requires_grad(false));
   const int64_t rows = update.size(-2), cols = update.size(-1), batch = update.numel() / (rows * cols);
-  const int code = dtype_code(what, update);
   const size_t bytes = enc_orthogonalize_workspace_bytes(code, batch, rows, cols);
   const Tensor ws = workspace(bytes, update);
   done(what, enc_orthogonalize(code, ptr(update), ptr(out), batch, rows, cols, (int)steps, (float)a, (float)b, (float)c, (float)eps, ptr(ws),
@@ -390,7 +397,8 @@ Tensor orthogonalize(const Tensor &given_update, int64_t steps, double a, double
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gated_feed_forward", &gated_feed_forward);
   m.def("residual_norm", &residual_norm);
-  m.def("orthogonalize", &orthogonalize);
+  m.def("orthogonalize", &orthogonalize, py::arg("update"), py::arg("steps"), py::arg("a"), py::arg("b"), py::arg("c"), py::arg("eps"),
+        py::arg("dtype") = py::none());
   // the checks alone, for the CPU path
   m.def("check_gated_feed_forward", [](const Tensor &x, const Tensor &w_in, const MaybeTensor &b_in, const Tensor &w_out, const MaybeTensor &b_out,
                                        const std::string &activation) {
@@ -404,6 +412,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     check_norm({x, y, given(gate), given(scale), given(inner_weight), given(inner_bias), given(outer_weight), given(outer_bias)},
                norm_code(inner), norm_code(outer), want_residual);
   });
-  m.def("check_orthogonalize", &check_orthogonalize);
+  m.def("check_orthogonalize", &check_orthogonalize, py::arg("update"), py::arg("steps"), py::arg("dtype") = py::none());
   m.def("launch_count", &enc_launch_count);
 }

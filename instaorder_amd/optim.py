@@ -8,14 +8,15 @@ COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
 @torch.no_grad()
-def orthogonalize(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
+def orthogonalize(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7, dtype=None):
     """The nearly orthogonal matrix that `steps` Newton-Schulz steps X <- a X + (b A + c A A) X, A = X X^T, make of
     update / max(|update|, eps) (Frobenius norm).  update [..., rows, cols], a batch of matrices of any shape, fp32, bf16
-    or fp16; the result has its shape and type.  Not differentiable.  A zero update gives zeros."""
+    or fp16; the result has its shape and type, or `dtype`: of an fp32 update bf16 or fp16 too (what the type does not reach
+    keeps its direction that way).  Not differentiable.  A zero update gives zeros."""
     a, b, c = coefficients
     if update.is_cuda:
-        return layer_ext.bind().orthogonalize(update, steps, a, b, c, eps)
-    layer_ext.bind().check_orthogonalize(update, steps)
+        return layer_ext.bind().orthogonalize(update, steps, a, b, c, eps, dtype)
+    layer_ext.bind().check_orthogonalize(update, steps, dtype)
     x = update.float()
     tall = x.shape[-2] > x.shape[-1]
     x = x.mT if tall else x
@@ -24,14 +25,15 @@ def orthogonalize(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     for _ in range(steps):
         gram = x @ x.mT
         x = a * x + (b * gram + c * (gram @ gram)) @ x
-    return (x.mT if tall else x).to(update.dtype).contiguous()
+    return (x.mT if tall else x).to(dtype or update.dtype).contiguous()
 
 
 class Muon(torch.optim.Optimizer):
     """For parameters of two dimensions (others: another optimiser).  v = momentum * v + g;  u = g + momentum * v (nesterov)
     or v;  w <- w (1 - lr * weight_decay) - lr * sqrt(max(1, rows / cols)) * orthogonalize(u).  Matrices of one shape,
     type and device are orthogonalised in one batch.  v and u are fp32 whatever the type of w (in 16 bits a gradient below
-    2^-9 of v would leave it as it is); u is rounded to w's type for its orthogonalisation, whose result has that type."""
+    2^-9 of v would leave it as it is, and u, up to 20 gradients, leaves fp16's range at either end); the orthogonal matrix
+    has w's type."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS,
                  eps=1e-7):
@@ -72,10 +74,10 @@ class Muon(torch.optim.Optimizer):
                 v = state["momentum_buffer"]
                 v.mul_(group["momentum"]).add_(p.grad)
                 u = p.grad.float().add(v, alpha=group["momentum"]) if group["nesterov"] else v
-                alike.setdefault((p.shape, p.dtype, p.device), []).append((p, u.to(p.dtype)))
-            for (shape, _, _), members in alike.items():
+                alike.setdefault((p.shape, p.dtype, p.device), []).append((p, u))
+            for (shape, dtype, _), members in alike.items():
                 batch = orthogonalize(torch.stack([u for _, u in members]), group["steps"], group["coefficients"],
-                                      group["eps"])
+                                      group["eps"], dtype)
                 factor = -group["lr"] * max(1.0, shape[0] / shape[1]) ** 0.5
                 for (p, _), o in zip(members, batch):
                     if group["weight_decay"]:

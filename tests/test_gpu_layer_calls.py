@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import layer_reference as R
-from test_gpu_layer import FLOATS, ffn_inputs, gen, norm_inputs, rand
+from test_gpu_layer import COEFFICIENTS, FLOATS, MUON, ffn_inputs, gen, norm_inputs, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,32 @@ def test_gates_shared_over_dimensions_of_one(dtype, lead, gate):
         size, steps = (w.abs().amax(-1, keepdim=True), 64) if v.shape == t["x"].shape else (w.abs().max(), 64 + 4 * rows ** 0.5)
         assert v.shape == w.shape and v.dtype == dtype
         R.within(v, w, (R.U[dtype] * w.abs()).clamp(min=R.FLOOR[dtype]) + steps * 16 * R.U32 * (size + 1.0) + R.TINY, k)
+
+
+# ---- Muon ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype, size", [(torch.float16, 9000.0), (torch.float16, 1.0), (torch.float16, 1e-5), (torch.float16, 2e-7),
+                                         (torch.bfloat16, 1e30), (torch.bfloat16, 1.0)])
+def test_muon_takes_gradients_of_any_size(dtype, size):
+    from test_layer_calls_cpu import MUON_16, muon_runs
+    got, want = muon_runs(dtype, size, "cuda")
+    assert got.isfinite().all()
+    assert float((got - want).norm() / want.norm()) <= MUON_16[dtype]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(1, 1), (7, 33), (3, 130, 65), (2, 260, 1000), (1500, 600), (0, 4, 4)])
+def test_orthogonalize_results_of_another_type(dtype, shape):
+    """An fp32 update with a 16-bit result: within the bound of that type, for values that the type does not reach too."""
+    from instaorder_amd import orthogonalize
+    u = rand(gen(5), *shape)
+    for factor in (1.0, 2.0 ** 40, 2.0 ** -10):
+        o = orthogonalize(u * factor, dtype=dtype)
+        assert o.shape == u.shape and o.dtype == dtype
+        if u.numel():
+            want = R.orthogonalize(u * factor, 5, COEFFICIENTS, 1e-7).flatten(-2)
+            off = (o.double().flatten(-2) - want).norm(dim=-1) / want.norm(dim=-1)
+            assert float(off.max()) <= MUON[dtype]
+    assert torch.equal(orthogonalize(u, dtype=torch.float32), orthogonalize(u))
+    for bad in (lambda: orthogonalize(u.to(dtype), dtype=torch.float32), lambda: orthogonalize(u, dtype=torch.float64)):
+        with pytest.raises(RuntimeError, match="orthogonalize"):
+            bad()

@@ -96,9 +96,63 @@ def test_every_failed_launch_of_the_attention_op_is_reported():
     assert handle.msda_launch_count() == before
 
 
+def muon_runs(dtype, size, device="cpu", steps=4):
+    """The same gradients, held exactly in `dtype`, for weights of that type and for fp32 weights: the two updates."""
+    from instaorder_amd import Muon
+    g = torch.Generator().manual_seed(11)
+    grads = [(torch.randn(24, 40, generator=g) * size).to(dtype) for _ in range(steps)]
+    out = []
+    for kind in (dtype, torch.float32):
+        p = torch.nn.Parameter(torch.zeros(24, 40, dtype=kind, device=device))
+        opt = Muon([p], lr=0.05)
+        for gr in grads:
+            p.data.zero_()                             # the update alone, not its sum with a rounded weight
+            p.grad = gr.to(device=device, dtype=kind)
+            opt.step()
+        out.append(p.detach().double().cpu())
+    return out
+
+
+# The update of 16-bit weights is off from that of fp32 weights by three roundings to the type of values up to 0.05 * 1.3 (the
+# orthogonal matrix, the product with the rate, the weight), on the GPU also by two-part iterates (485 * 2^-17, as derived
+# in test_gpu_layer.py); in the 2-norm of the whole the largest a rounding can be.
+MUON_16 = {torch.float16: 3 * 2.0 ** -11 + 485 * 2.0 ** -17, torch.bfloat16: 3 * 2.0 ** -8 + 485 * 2.0 ** -17}
+
+
+@pytest.mark.parametrize("dtype, size", [(torch.float16, 9000.0), (torch.float16, 1.0), (torch.float16, 1e-5), (torch.float16, 2e-7),
+                                         (torch.bfloat16, 1e30), (torch.bfloat16, 1.0)])
+def test_muon_takes_gradients_of_any_size(dtype, size):
+    """v + g grows to 20 times the gradient and leaves fp16's range at either end; its direction is all that counts."""
+    got, want = muon_runs(dtype, size)
+    assert got.isfinite().all()
+    assert float((got - want).norm() / want.norm()) <= MUON_16[dtype]
+
+
+def test_orthogonalize_results_of_another_type():
+    from instaorder_amd import orthogonalize
+    u = torch.randn(2, 6, 9, generator=torch.Generator().manual_seed(2)) * 1e30
+    for dtype in (torch.float16, torch.bfloat16, torch.float32):
+        o = orthogonalize(u, dtype=dtype)
+        assert o.dtype == dtype and torch.equal(o, orthogonalize(u).to(dtype))
+    for given, dtype in ((torch.float16, torch.float32), (torch.float16, torch.bfloat16), (torch.float32, torch.float64),
+                         (torch.bfloat16, torch.int16)):
+        with pytest.raises(RuntimeError, match="orthogonalize"):
+            orthogonalize(u.to(given), dtype=dtype)
+
+
 @pytest.mark.parametrize("factor", [2.0 ** -60, 2.0 ** 100])
 def test_cpu_orthogonalize_of_values_whose_squares_leave_32_bits(factor):
     from instaorder_amd import orthogonalize
     u = torch.randn(2, 6, 9, generator=torch.Generator().manual_seed(2))
     want = orthogonalize(u)
     assert torch.allclose(orthogonalize(u * factor, eps=1e-30), want, rtol=1e-5, atol=1e-6)
+
+
+@pytest.mark.parametrize("dtype, text", [(16, "unknown dtype"), (17, "workspace"), (18, "workspace"), (19, "unknown dtype")])
+def test_c_abi_types_of_an_fp32_update(dtype, text):
+    from test_layer_cpu import lib
+    handle = lib()
+    assert handle.enc_orthogonalize(dtype, 256, 256, 2, 8, 8, 5, 1.0, 1.0, 1.0, 1e-7, None, 0, None) == 1
+    assert text in handle.enc_last_error().decode()
+    room = handle.enc_orthogonalize_workspace_bytes
+    assert room(dtype, 2, 8, 8) == (room(dtype & 3, 2, 8, 8) if text == "workspace" else 0)
