@@ -41,10 +41,13 @@ class Muon(torch.optim.Optimizer):
             raise ValueError("Muon: lr and weight_decay must not be negative, momentum must be in [0, 1)")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
                                       coefficients=coefficients, eps=eps))
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() != 2:
-                    raise ValueError("Muon takes parameters of two dimensions, got one of shape %s" % (tuple(p.shape),))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)          # (the constructor's groups come this way too)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() != 2:
+                del self.param_groups[-1]
+                raise ValueError("Muon takes parameters of two dimensions, got one of shape %s" % (tuple(p.shape),))
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)           # casts to the parameters' types

@@ -156,3 +156,15 @@ def test_c_abi_types_of_an_fp32_update(dtype, text):
     assert text in handle.enc_last_error().decode()
     room = handle.enc_orthogonalize_workspace_bytes
     assert room(dtype, 2, 8, 8) == (room(dtype & 3, 2, 8, 8) if text == "workspace" else 0)
+
+
+@pytest.mark.parametrize("shape", [(6,), (2, 3, 4), ()])
+def test_muon_refuses_added_groups_of_other_dimensions(shape):
+    """A group that is added later: biases of one shape would be taken for the rows of a matrix."""
+    from instaorder_amd import Muon
+    opt = Muon([torch.nn.Parameter(torch.zeros(3, 3))])
+    with pytest.raises(ValueError, match="two dimensions"):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(shape))]})
+    assert len(opt.param_groups) == 1
+    opt.add_param_group({"params": torch.nn.Parameter(torch.zeros(4, 3)), "lr": 0.1})
+    assert len(opt.param_groups) == 2
