@@ -22,9 +22,10 @@ def orthogonalize(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7, dtype=No
     x = x.mT if tall else x
     norm = x.double().square().sum((-2, -1), keepdim=True).sqrt()        # squares of 32-bit values leave 32 bits
     x = (x / norm.clamp(min=eps)).float()
-    for _ in range(steps):
-        gram = x @ x.mT
-        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    with torch.autocast("cpu", enabled=False):
+        for _ in range(steps):
+            gram = x @ x.mT
+            x = a * x + (b * gram + c * (gram @ gram)) @ x
     return (x.mT if tall else x).to(dtype or update.dtype).contiguous()
 
 

@@ -168,3 +168,11 @@ def test_muon_refuses_added_groups_of_other_dimensions(shape):
     assert len(opt.param_groups) == 1
     opt.add_param_group({"params": torch.nn.Parameter(torch.zeros(4, 3)), "lr": 0.1})
     assert len(opt.param_groups) == 2
+
+
+def test_cpu_orthogonalize_is_the_same_under_autocast():
+    from instaorder_amd import orthogonalize
+    u = torch.randn(12, 20, generator=torch.Generator().manual_seed(4))
+    want = orthogonalize(u)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        assert torch.equal(orthogonalize(u), want)
