@@ -21,7 +21,7 @@ from torch import nn
 from torch.nn.init import normal_
 
 from . import layer_ext
-from .layer import ACTIVATIONS, gated_feed_forward, residual_norm
+from .layer import ACTIVATIONS, autocast_dtype, gated_feed_forward, residual_norm
 from .modules import MSDeformAttn
 
 
@@ -86,9 +86,15 @@ class MSDeformAttnTransformerEncoderLayer(nn.Module):
             nn.init.zeros_(self.adapter[2].weight)
             nn.init.zeros_(self.adapter[2].bias)
 
+    @staticmethod
+    def _one_type(*tensors):
+        """Of one type that the layer operators take, or of any of them under autocast, which they follow."""
+        return (all(t.dtype in layer_ext.DTYPES for t in tensors)
+                and (len({t.dtype for t in tensors}) == 1 or autocast_dtype(tensors[0]) is not None))
+
     def _add_and_norm(self, src, block, norm):
-        if (self.fused_norm and src.is_cuda and src.dtype in layer_ext.DTYPES
-                and src.dtype == block.dtype == norm.weight.dtype and src.shape[-1] <= layer_ext.NORM_MAX_WIDTH):
+        if (self.fused_norm and src.is_cuda and self._one_type(src, block, norm.weight)
+                and src.shape[-1] <= layer_ext.NORM_MAX_WIDTH):
             return residual_norm(src, block, outer="layer", outer_weight=norm.weight, outer_bias=norm.bias, eps=norm.eps,
                                  want_residual=False)[1]
         return norm(src + block)
@@ -97,7 +103,7 @@ class MSDeformAttnTransformerEncoderLayer(nn.Module):
         if not self.gate:
             return self.linear2(self.dropout2(self.activation(self.linear1(src))))
         dropping = self.training and self.dropout2.p > 0
-        if dropping or src.dtype not in layer_ext.DTYPES or src.dtype != self.linear1.weight.dtype:
+        if dropping or not self._one_type(src, self.linear1.weight):
             value, gate = self.linear1(src).chunk(2, -1)
             return self.linear2(self.dropout2(value * self.activation(gate)))
         return gated_feed_forward(src, self.linear1.weight, self.linear1.bias, self.linear2.weight, self.linear2.bias,

@@ -15,6 +15,17 @@ from . import layer_ext
 ACTIVATIONS = {"silu": F.silu, "gelu": F.gelu, "sigmoid": torch.sigmoid, "relu": F.relu}
 
 
+def autocast_dtype(x):
+    """The type that autocast runs products in on x's device, None where it is off."""
+    device = "cuda" if x.is_cuda else "cpu"
+    return torch.get_autocast_dtype(device) if torch.is_autocast_enabled(device) else None
+
+
+def _cast(tensors, dtype):
+    """What autocast casts: floating point tensors below 64 bits.  (Each call casts for itself: nothing is kept.)"""
+    return [t.to(dtype) if t is not None and t.is_floating_point() and t.dtype != torch.float64 else t for t in tensors]
+
+
 def gated_feed_forward(x, w_in, b_in, w_out, b_out, activation="silu"):
     """y = (a * act(b)) W_out^T + b_out with [a | b] = x W_in^T + b_in.
 
@@ -23,13 +34,17 @@ def gated_feed_forward(x, w_in, b_in, w_out, b_out, activation="silu"):
     fp32, bf16 or fp16, one type for all; sums are fp32, h is rounded to the type once.  Differentiable once in all five
     tensors.  fp32 goes through three bf16 parts in the backward pass and in forward passes of many tokens: there an Inf among
     the inputs gives NaN (its parts multiply zeros), a NaN stays one, and values below 2^-110 lose their low bits (their
-    parts end at 2^-133)."""
+    parts end at 2^-133).  Under autocast all five are cast to its type, as for ``F.linear``."""
+    dtype = autocast_dtype(x)
+    if dtype is not None:
+        x, w_in, b_in, w_out, b_out = _cast((x, w_in, b_in, w_out, b_out), dtype)
     bind = layer_ext._bind or layer_ext.bind()
     if x.is_cuda:
         return bind.gated_feed_forward(x, w_in, b_in, w_out, b_out, activation)
     bind.check_gated_feed_forward(x, w_in, b_in, w_out, b_out, activation)
-    a, b = F.linear(x, w_in, b_in).chunk(2, -1)
-    return F.linear(a * ACTIVATIONS[activation](b), w_out, b_out)
+    with torch.autocast("cpu", enabled=False):
+        a, b = F.linear(x, w_in, b_in).chunk(2, -1)
+        return F.linear(a * ACTIVATIONS[activation](b), w_out, b_out)
 
 
 def _cpu_norm(v, kind, weight, bias, eps):
@@ -50,7 +65,10 @@ def residual_norm(x, y, *, gate=None, scale=None, inner=None, inner_weight=None,
     optional weight and bias [width]; scale [width]; gate of x's shape, or with ones in its last dimensions before the
     width (x [batch, tokens, width], gate [batch, 1, width]: one gate for a sample).  want_residual=False leaves the
     residual in registers.  fp32, bf16 or fp16, one type for all; fp32 inside, each result rounded once.  Differentiable
-    once in all eight tensors."""
+    once in all eight tensors.  Under autocast all are cast to fp32, as for ``F.layer_norm``."""
+    if autocast_dtype(x) is not None:
+        x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias = _cast(
+            (x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias), torch.float32)
     bind = layer_ext._bind or layer_ext.bind()
     if x.is_cuda:
         return bind.residual_norm(x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias, eps,

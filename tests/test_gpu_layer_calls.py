@@ -51,6 +51,34 @@ def test_gates_shared_over_dimensions_of_one(dtype, lead, gate):
         R.within(v, w, (R.U[dtype] * w.abs()).clamp(min=R.FLOOR[dtype]) + steps * 16 * R.U32 * (size + 1.0) + R.TINY, k)
 
 
+# ---- autocast -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_operators_under_autocast(dtype):
+    from test_layer_calls_cpu import autocast_checks
+    autocast_checks("cuda", dtype)
+
+
+@pytest.mark.parametrize("activation", ["relu", "swiglu"])
+def test_fused_norm_of_the_layer_under_autocast(activation):
+    """A 16-bit block under an fp32 residual goes through the kernel, with the values of the plain path."""
+    from instaorder_amd import layer_ext
+    from instaorder_amd.encoder import MSDeformAttnTransformerEncoderLayer
+    torch.manual_seed(0)
+    layer = MSDeformAttnTransformerEncoderLayer(64, 96, 0.0, activation, n_levels=1, n_heads=2, n_points=4).cuda()
+    src = rand(gen(1), 2, 130, 64)
+    out = {}
+    for fused in (False, True):
+        layer.fused_norm = fused
+        before = layer_ext.launch_count()
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            out[fused] = layer._add_and_norm(src, layer._feed_forward(src), layer.norm2)
+        launches = layer_ext.launch_count() - before
+        assert out[fused].dtype == torch.float32 and (launches > 0) == (fused or activation != "relu")
+    assert launches > (activation != "relu")
+    # the same 16-bit block: the norms' sums in another order
+    assert float((out[True] - out[False]).abs().max()) <= 64 * R.U32 * 16 * (1 + float(out[False].abs().max()))
+
+
 # ---- Muon ---------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype, size", [(torch.float16, 9000.0), (torch.float16, 1.0), (torch.float16, 1e-5), (torch.float16, 2e-7),
                                          (torch.bfloat16, 1e30), (torch.bfloat16, 1.0)])

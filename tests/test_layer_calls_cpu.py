@@ -170,9 +170,62 @@ def test_muon_refuses_added_groups_of_other_dimensions(shape):
     assert len(opt.param_groups) == 2
 
 
+def autocast_checks(device, dtype):
+    """Under autocast the block runs in autocast's type, as F.linear does, and the norm in fp32, as F.layer_norm does: the
+    calls of tensors cast by hand; gradients arrive in the leaves' own types."""
+    from instaorder_amd import gated_feed_forward, residual_norm
+    g = torch.Generator().manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g).to(device)      # noqa: E731
+    x, wi, bi, wo, bo = (v.requires_grad_(True) for v in (r(3, 5, 16), r(48, 16), r(48), r(16, 24), r(16)))
+    for given in (x, x.to(dtype)):
+        with torch.autocast(device, dtype=dtype):
+            y = gated_feed_forward(given, wi, bi, wo, bo)
+        want = gated_feed_forward(*[v.to(dtype) for v in (x, wi, bi, wo, bo)])
+        assert y.dtype == dtype and torch.equal(y, want)
+        pull = r(3, 5, 16).to(dtype)
+        got = torch.autograd.grad(y, [x, wi, bi, wo, bo], pull)
+        ref = torch.autograd.grad(want, [x, wi, bi, wo, bo], pull)
+        assert all(a.dtype == torch.float32 and torch.equal(a, b) for a, b in zip(got, ref))
+    w, b, gate = (v.requires_grad_(True) for v in (r(16), r(16), r(3, 1, 16)))
+    block = y.detach().requires_grad_(True)             # a 16-bit block under an fp32 residual
+    for given in (x, x.to(dtype)):
+        with torch.autocast(device, dtype=dtype):
+            res, n = residual_norm(given, block, gate=gate, inner="rms", outer="layer", outer_weight=w, outer_bias=b)
+        want = residual_norm(given.float(), block.float(), gate=gate, inner="rms", outer="layer", outer_weight=w, outer_bias=b)
+        assert all(a.dtype == torch.float32 and torch.equal(a, c) for a, c in zip((res, n), want))
+        got = torch.autograd.grad([res.sum(), n.square().sum()], [x, block, gate, w, b])
+        ref = torch.autograd.grad([want[0].sum(), want[1].square().sum()], [x, block, gate, w, b])
+        assert all(a.dtype == c.dtype and torch.equal(a, c) for a, c in zip(got, ref)) and got[1].dtype == dtype
+    with torch.autocast(device, dtype=dtype), pytest.raises(RuntimeError, match="not implemented for"):
+        gated_feed_forward(x.double(), wi, bi, wo, bo)   # 64 bits stay what they are
+    with torch.autocast(device, enabled=False), pytest.raises(RuntimeError, match="has dtype"):
+        gated_feed_forward(x.to(dtype), wi, bi, wo, bo)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_operators_under_autocast(dtype):
+    autocast_checks("cpu", dtype)
+
+
 def test_cpu_orthogonalize_is_the_same_under_autocast():
     from instaorder_amd import orthogonalize
     u = torch.randn(12, 20, generator=torch.Generator().manual_seed(4))
     want = orthogonalize(u)
     with torch.autocast("cpu", dtype=torch.bfloat16):
         assert torch.equal(orthogonalize(u), want)
+
+
+def encoder_layer(activation, dropout=0.0):
+    from instaorder_amd.encoder import MSDeformAttnTransformerEncoderLayer
+    torch.manual_seed(0)
+    return MSDeformAttnTransformerEncoderLayer(32, 24, dropout, activation, n_levels=1, n_heads=4, n_points=2)
+
+
+def test_gated_block_of_the_layer_under_autocast():
+    layer, x = encoder_layer("swiglu"), torch.randn(2, 5, 32)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        got = layer._feed_forward(x)
+        a, b = layer.linear1(x).chunk(2, -1)
+        plain = layer.linear2(a * torch.nn.functional.silu(b))
+    assert got.dtype == plain.dtype == torch.bfloat16
+    assert torch.allclose(got.float(), plain.float(), atol=4 * 2.0 ** -8 * float(plain.abs().max()))
