@@ -19,6 +19,7 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 from torch.nn.init import normal_
+from torch.nn.modules.module import _has_any_global_hook
 
 from . import layer_ext
 from .layer import ACTIVATIONS, autocast_dtype, gated_feed_forward, residual_norm
@@ -61,6 +62,14 @@ def _activation(name):
     return {"relu": F.relu, "gelu": F.gelu, **{k: ACTIVATIONS[v] for k, v in GATED.items()}}[name]
 
 
+def _as_made(module, kind):
+    """Does calling `module` do what `kind` does and nothing else?  Not for a subclass or a wrapper (an adapter, a
+    parametrisation), a forward of its own, or one with hooks: those have to be called."""
+    return (type(module) is kind and "forward" not in module.__dict__
+            and not (module._forward_pre_hooks or module._forward_hooks or module._backward_pre_hooks
+                     or module._backward_hooks or _has_any_global_hook()))
+
+
 class MSDeformAttnTransformerEncoderLayer(nn.Module):
     def __init__(self, d_model=256, d_ffn=1024, dropout=0.1, activation="relu", n_levels=4,
                  n_heads=8, n_points=4, use_adapters=False, adapter_dim=64, adapter_scale=0.1):
@@ -75,7 +84,8 @@ class MSDeformAttnTransformerEncoderLayer(nn.Module):
         self.linear2 = nn.Linear(d_ffn, d_model)
         self.dropout3 = nn.Dropout(dropout)
         self.norm2 = nn.LayerNorm(d_model)
-        # opt-in (not reference behaviour): src + block and its norm in one kernel (residual_norm)
+        # opt-in (not reference behaviour): src + block and its norm in one kernel (residual_norm).  Like the gated block's
+        # kernels it takes the place of submodules that are as they were made; others (hooks, wrappers) are called.
         self.fused_norm = False
         self.use_adapters, self.adapter_scale = use_adapters, adapter_scale
         if use_adapters:        # InstaFormer's trainable adapters (msdeformattn.py:155-166)
@@ -93,7 +103,8 @@ class MSDeformAttnTransformerEncoderLayer(nn.Module):
                 and (len({t.dtype for t in tensors}) == 1 or autocast_dtype(tensors[0]) is not None))
 
     def _add_and_norm(self, src, block, norm):
-        if (self.fused_norm and src.is_cuda and self._one_type(src, block, norm.weight)
+        if (self.fused_norm and src.is_cuda and _as_made(norm, nn.LayerNorm) and norm.normalized_shape == src.shape[-1:]
+                and self._one_type(src, block, *([] if norm.weight is None else [norm.weight]))
                 and src.shape[-1] <= layer_ext.NORM_MAX_WIDTH):
             return residual_norm(src, block, outer="layer", outer_weight=norm.weight, outer_bias=norm.bias, eps=norm.eps,
                                  want_residual=False)[1]
@@ -102,8 +113,10 @@ class MSDeformAttnTransformerEncoderLayer(nn.Module):
     def _feed_forward(self, src):
         if not self.gate:
             return self.linear2(self.dropout2(self.activation(self.linear1(src))))
-        dropping = self.training and self.dropout2.p > 0
-        if dropping or not self._one_type(src, self.linear1.weight):
+        made = (_as_made(self.linear1, nn.Linear) and _as_made(self.linear2, nn.Linear) and _as_made(self.dropout2, nn.Dropout)
+                and self.activation is ACTIVATIONS[self.gate])
+        dropping = self.dropout2.training and self.dropout2.p > 0        # dropout of h: inside the block, not in the kernels
+        if not made or dropping or not self._one_type(src, self.linear1.weight):
             value, gate = self.linear1(src).chunk(2, -1)
             return self.linear2(self.dropout2(value * self.activation(gate)))
         return gated_feed_forward(src, self.linear1.weight, self.linear1.bias, self.linear2.weight, self.linear2.bias,

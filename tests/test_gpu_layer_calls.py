@@ -79,6 +79,42 @@ def test_fused_norm_of_the_layer_under_autocast(activation):
     assert float((out[True] - out[False]).abs().max()) <= 64 * R.U32 * 16 * (1 + float(out[False].abs().max()))
 
 
+# ---- submodules of the layer ----------------------------------------------------------------------
+def test_changed_norms_of_the_layer_are_called():
+    from instaorder_amd import layer_ext
+    from instaorder_amd.encoder import MSDeformAttnTransformerEncoderLayer
+    torch.manual_seed(0)
+    layer = MSDeformAttnTransformerEncoderLayer(64, 96, 0.0, "relu", n_levels=1, n_heads=2, n_points=4).cuda()
+    layer.fused_norm = True
+    src, block = rand(gen(1), 2, 30, 64), rand(gen(2), 2, 30, 64)
+
+    def call():
+        before = layer_ext.launch_count()
+        out = layer._add_and_norm(src, block, layer.norm1)
+        return out.detach(), layer_ext.launch_count() > before
+
+    plain, fused = call()
+    assert fused
+    handle = layer.norm1.register_forward_hook(lambda m, i, o: o * 3)
+    out, fused = call()
+    assert not fused and torch.allclose(out, 3 * plain, atol=1e-4)
+    handle.remove()
+    layer.norm1 = torch.nn.LayerNorm(64, elementwise_affine=False).cuda()        # no weight: still the kernel
+    out, fused = call()
+    assert fused and torch.allclose(out, plain, atol=1e-4)                       # (the weights were still one and zero)
+    layer.norm1 = torch.nn.LayerNorm((30, 64)).cuda()                            # over two dimensions: not the kernel's norm
+    out, fused = call()
+    assert not fused and torch.equal(out, layer.norm1(src + block))
+
+    class Doubled(torch.nn.LayerNorm):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    layer.norm1 = Doubled(64).cuda()
+    out, fused = call()
+    assert not fused and torch.allclose(out, 2 * plain, atol=1e-4)
+
+
 # ---- Muon ---------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype, size", [(torch.float16, 9000.0), (torch.float16, 1.0), (torch.float16, 1e-5), (torch.float16, 2e-7),
                                          (torch.bfloat16, 1e30), (torch.bfloat16, 1.0)])

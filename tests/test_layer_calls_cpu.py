@@ -229,3 +229,61 @@ def test_gated_block_of_the_layer_under_autocast():
         plain = layer.linear2(a * torch.nn.functional.silu(b))
     assert got.dtype == plain.dtype == torch.bfloat16
     assert torch.allclose(got.float(), plain.float(), atol=4 * 2.0 ** -8 * float(plain.abs().max()))
+
+
+def submodule_changes():
+    """(what, change(layer)): each replaces or watches a submodule of the gated block; a call has to show it."""
+    def own_forward(layer):
+        inner = layer.linear1.forward
+        layer.linear1.forward = lambda x: 2 * inner(x)
+
+    class Wrapped(torch.nn.Module):
+        def __init__(self, inner):
+            super().__init__()
+            self.inner, self.weight, self.bias = inner, inner.weight, inner.bias
+
+        def forward(self, x):
+            return self.inner(x) + 1
+
+    class Doubled(torch.nn.Linear):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    def subclass(layer):
+        new = Doubled(24, 32)
+        new.load_state_dict(layer.linear2.state_dict())
+        layer.linear2 = new
+
+    return [("hook on the output", lambda layer: layer.linear1.register_forward_hook(lambda m, i, o: o * 3)),
+            ("hook on the input", lambda layer: layer.linear2.register_forward_pre_hook(lambda m, i: (i[0] + 1,))),
+            ("hook on dropout", lambda layer: layer.dropout2.register_forward_hook(lambda m, i, o: o * 3)),
+            ("forward of its own", own_forward), ("wrapper", lambda layer: setattr(layer, "linear2", Wrapped(layer.linear2))),
+            ("subclass", subclass), ("activation", lambda layer: setattr(layer, "activation", torch.tanh)),
+            ("dropout alone in training", lambda layer: (layer.eval(), setattr(layer.dropout2, "p", 0.9), layer.dropout2.train()))]
+
+
+@pytest.mark.parametrize("at", range(8))
+def test_changed_submodules_of_the_gated_block_are_called(at):
+    what, change = submodule_changes()[at]
+    layer, x = encoder_layer("swiglu"), torch.randn(2, 5, 32)
+    plain = layer._feed_forward(x)
+    change(layer)
+    torch.manual_seed(3)
+    got = layer._feed_forward(x)
+    torch.manual_seed(3)
+    a, b = layer.linear1(x).chunk(2, -1)
+    want = layer.linear2(layer.dropout2(a * layer.activation(b)))
+    assert torch.equal(got, want) and not torch.allclose(got, plain), what
+
+
+def test_hooks_of_all_modules_and_of_gradients_see_the_gated_block():
+    layer, x, seen = encoder_layer("swiglu"), torch.randn(2, 5, 32), []
+    handle = torch.nn.modules.module.register_module_forward_hook(lambda m, i, o: seen.append(m))
+    try:
+        layer._feed_forward(x)
+    finally:
+        handle.remove()
+    assert layer.linear1 in seen and layer.linear2 in seen
+    layer.linear1.register_full_backward_hook(lambda m, gi, go: seen.clear())
+    layer._feed_forward(x).sum().backward()
+    assert not seen
