@@ -64,8 +64,9 @@ def _activation(name):
 
 def _as_made(module, kind):
     """Does calling `module` do what `kind` does and nothing else?  Not for a subclass or a wrapper (an adapter, a
-    parametrisation), a forward of its own, or one with hooks: those have to be called."""
-    return (type(module) is kind and "forward" not in module.__dict__
+    parametrisation), a forward of its own, or one with hooks: those have to be called.  Nor under torch.jit.trace, which
+    records torch's own operators and refuses the kernels."""
+    return (type(module) is kind and "forward" not in module.__dict__ and not torch.jit.is_tracing()
             and not (module._forward_pre_hooks or module._forward_hooks or module._backward_pre_hooks
                      or module._backward_hooks or _has_any_global_hook()))
 

@@ -115,6 +115,24 @@ def test_changed_norms_of_the_layer_are_called():
     assert not fused and torch.allclose(out, 2 * plain, atol=1e-4)
 
 
+@pytest.mark.parametrize("activation", ["relu", "swiglu"])
+def test_traced_layer_takes_its_modules(activation):
+    from instaorder_amd.encoder import MSDeformAttnTransformerEncoderLayer
+    torch.manual_seed(0)
+    layer = MSDeformAttnTransformerEncoderLayer(64, 96, 0.0, activation, n_levels=1, n_heads=2, n_points=4).cuda()
+    layer.requires_grad_(False)                          # a trace of a function takes weights as constants
+    layer.fused_norm = True
+
+    def call(x):
+        return layer._add_and_norm(x, layer._feed_forward(x), layer.norm2)
+
+    with torch.no_grad():
+        traced = torch.jit.trace(call, rand(gen(1), 2, 30, 64))
+        for seed in (1, 2):
+            x = rand(gen(seed), 2, 30, 64)
+            assert torch.allclose(traced(x), call(x), atol=1e-4)
+
+
 # ---- Muon ---------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype, size", [(torch.float16, 9000.0), (torch.float16, 1.0), (torch.float16, 1e-5), (torch.float16, 2e-7),
                                          (torch.bfloat16, 1e30), (torch.bfloat16, 1.0)])
