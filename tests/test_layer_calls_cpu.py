@@ -287,3 +287,13 @@ def test_hooks_of_all_modules_and_of_gradients_see_the_gated_block():
     layer.linear1.register_full_backward_hook(lambda m, gi, go: seen.clear())
     layer._feed_forward(x).sum().backward()
     assert not seen
+
+
+def test_layers_saved_whole_before_the_gated_block_still_run():
+    """A pickled layer has its attributes, not those that later ones set in their constructor."""
+    layer, x = encoder_layer("relu"), torch.randn(1, 12, 32)
+    args = (None, torch.rand(1, 12, 1, 2), torch.tensor([[3, 4]]), torch.tensor([0]))
+    want = layer(x, *args)
+    for name in ("gate", "fused_norm"):
+        layer.__dict__.pop(name, None)
+    assert torch.equal(layer(x, *args), want)
