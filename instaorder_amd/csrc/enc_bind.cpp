@@ -399,19 +399,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("residual_norm", &residual_norm);
   m.def("orthogonalize", &orthogonalize, py::arg("update"), py::arg("steps"), py::arg("a"), py::arg("b"), py::arg("c"), py::arg("eps"),
         py::arg("dtype") = py::none());
-  // the checks alone, for the CPU path
-  m.def("check_gated_feed_forward", [](const Tensor &x, const Tensor &w_in, const MaybeTensor &b_in, const Tensor &w_out, const MaybeTensor &b_out,
-                                       const std::string &activation) {
-    activation_code(activation);
-    check_ffn(x, w_in, given(b_in), w_out, given(b_out));
-  });
-  m.def("check_residual_norm", [](const Tensor &x, const Tensor &y, const MaybeTensor &gate, const MaybeTensor &scale,
-                                  const std::optional<std::string> &inner, const MaybeTensor &inner_weight, const MaybeTensor &inner_bias,
-                                  const std::optional<std::string> &outer, const MaybeTensor &outer_weight, const MaybeTensor &outer_bias,
-                                  bool want_residual) {
-    check_norm({x, y, given(gate), given(scale), given(inner_weight), given(inner_bias), given(outer_weight), given(outer_bias)},
-               norm_code(inner), norm_code(outer), want_residual);
-  });
-  m.def("check_orthogonalize", &check_orthogonalize, py::arg("update"), py::arg("steps"), py::arg("dtype") = py::none());
   m.def("launch_count", &enc_launch_count);
 }

@@ -73,6 +73,7 @@ def _as_made(module, kind):
 
 class MSDeformAttnTransformerEncoderLayer(nn.Module):
     gate, fused_norm = None, False      # of a layer that was pickled whole before it had them
+
     def __init__(self, d_model=256, d_ffn=1024, dropout=0.1, activation="relu", n_levels=4,
                  n_heads=8, n_points=4, use_adapters=False, adapter_dim=64, adapter_scale=0.1):
         super().__init__()

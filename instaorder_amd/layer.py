@@ -10,7 +10,7 @@ tensors, whose tangents the kernels do not carry."""
 import torch
 import torch.nn.functional as F
 
-from . import layer_ext
+from . import layer_checks, layer_ext
 
 ACTIVATIONS = {"silu": F.silu, "gelu": F.gelu, "sigmoid": torch.sigmoid, "relu": F.relu}
 
@@ -38,10 +38,9 @@ def gated_feed_forward(x, w_in, b_in, w_out, b_out, activation="silu"):
     dtype = autocast_dtype(x)
     if dtype is not None:
         x, w_in, b_in, w_out, b_out = _cast((x, w_in, b_in, w_out, b_out), dtype)
-    bind = layer_ext._bind or layer_ext.bind()
     if x.is_cuda:
-        return bind.gated_feed_forward(x, w_in, b_in, w_out, b_out, activation)
-    bind.check_gated_feed_forward(x, w_in, b_in, w_out, b_out, activation)
+        return (layer_ext._bind or layer_ext.bind()).gated_feed_forward(x, w_in, b_in, w_out, b_out, activation)
+    layer_checks.gated_feed_forward(x, w_in, b_in, w_out, b_out, activation, ACTIVATIONS)
     with torch.autocast("cpu", enabled=False):
         a, b = F.linear(x, w_in, b_in).chunk(2, -1)
         return F.linear(a * ACTIVATIONS[activation](b), w_out, b_out)
@@ -69,11 +68,10 @@ def residual_norm(x, y, *, gate=None, scale=None, inner=None, inner_weight=None,
     if autocast_dtype(x) is not None:
         x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias = _cast(
             (x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias), torch.float32)
-    bind = layer_ext._bind or layer_ext.bind()
     if x.is_cuda:
-        return bind.residual_norm(x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias, eps,
-                                  want_residual)
-    bind.check_residual_norm(x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias, want_residual)
+        return (layer_ext._bind or layer_ext.bind()).residual_norm(x, y, gate, scale, inner, inner_weight, inner_bias, outer,
+                                                                   outer_weight, outer_bias, eps, want_residual)
+    layer_checks.residual_norm(x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias, want_residual)
     z = y if inner is None else _cpu_norm(y, inner, inner_weight, inner_bias, eps)
     z = z if gate is None else z * gate
     r = x + (z if scale is None else z * scale)

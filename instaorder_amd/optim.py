@@ -2,7 +2,7 @@
 operation itself (GPU: the kernels of libenc_hip.so; CPU tensors: an elementary PyTorch path, by device)."""
 import torch
 
-from . import layer_ext
+from . import layer_checks, layer_ext
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
@@ -16,7 +16,7 @@ def orthogonalize(update, steps=5, coefficients=COEFFICIENTS, eps=1e-7, dtype=No
     a, b, c = coefficients
     if update.is_cuda:
         return layer_ext.bind().orthogonalize(update, steps, a, b, c, eps, dtype)
-    layer_ext.bind().check_orthogonalize(update, steps, dtype)
+    layer_checks.orthogonalize(update, steps, dtype)
     x = update.float()
     tall = x.shape[-2] > x.shape[-1]
     x = x.mT if tall else x

@@ -297,3 +297,86 @@ def test_layers_saved_whole_before_the_gated_block_still_run():
     for name in ("gate", "fused_norm"):
         layer.__dict__.pop(name, None)
     assert torch.equal(layer(x, *args), want)
+
+
+def test_cpu_paths_need_no_build(tmp_path):
+    """Only GPU tensors need the compiled library: a copy of the package without it computes on the CPU and says what a GPU
+    call would need."""
+    import os
+    import shutil
+    import subprocess
+    import sys
+    from conftest import ROOT
+    shutil.copytree(os.path.join(ROOT, "instaorder_amd"), tmp_path / "instaorder_amd",
+                    ignore=shutil.ignore_patterns("*.so", "*.o", "__pycache__", "csrc"))
+    code = """
+import torch, instaorder_amd as A
+x, w, v = torch.randn(3, 8), torch.randn(12, 8), torch.randn(8, 6)
+assert A.gated_feed_forward(x, w, None, v, None).shape == (3, 8)
+assert A.residual_norm(x, x)[1].shape == (3, 8)
+assert A.orthogonalize(x).shape == (3, 8)
+p = torch.nn.Parameter(x); p.grad = x.clone(); A.Muon([p]).step()
+for call in (lambda: A.gated_feed_forward(x, w[1:], None, v, None), lambda: A.residual_norm(x, x[:, 1:])):
+    try:
+        call()
+        raise SystemExit("taken")
+    except RuntimeError as e:
+        assert "shape" in str(e) or "expected" in str(e), e
+from instaorder_amd import layer_ext
+try:
+    layer_ext.bind()
+    raise SystemExit("bound")
+except RuntimeError as e:
+    assert "not built" in str(e)
+print("ok")
+"""
+    run = subprocess.run([sys.executable, "-c", code], cwd=tmp_path, capture_output=True, text=True, timeout=300,
+                         env=dict(os.environ, PYTHONPATH=str(tmp_path)))
+    assert run.returncode == 0 and run.stdout.strip() == "ok", run.stderr[-2000:]
+
+
+def refusals():
+    """Calls that both the CPU paths and the kernels' binding refuse: (operator, arguments)."""
+    g = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g)      # noqa: E731
+    x, wi, bi, wo, bo = r(2, 3, 8), r(12, 8), r(12), r(5, 6), r(5)
+    ffn = [(x, wi, bi, wo, bo, "tanh"), (x.double(), wi, bi, wo, bo, "silu"), (x.long(), wi, bi, wo, bo, "silu"),
+           (x, wi[:-1], bi, wo, bo, "silu"), (x, wi[:, 1:], bi, wo, bo, "silu"), (x, wi[0], bi, wo, bo, "silu"),
+           (x, wi, bi, wo[0], bo, "silu"), (x, wi, bi[1:], wo, bo, "silu"), (x, wi, bi, wo.half(), bo, "silu"),
+           (x, wi, bi, wo, bo[1:], "silu"), (x, wi.to("meta"), bi, wo, bo, "silu"), (x[..., :0], wi[:, :0], bi, wo, bo, "silu"),
+           (x, wi[:0], bi[:0], wo[:, :0], bo, "silu"), (torch.tensor(1.0), wi, bi, wo, bo, "silu")]
+    n = lambda x, y, gate=None, scale=None, inner=None, iw=None, ib=None, outer="layer", ow=None, ob=None, want=True: (      # noqa: E731
+        x, y, gate, scale, inner, iw, ib, outer, ow, ob, 1e-5, want)
+    norm = [n(x, x[..., 1:]), n(x, x, inner="batch"), n(x, x, outer="l2"), n(x, x, outer=None, want=False), n(x, x, iw=x[0, 0]),
+            n(x, x, ib=x[0, 0]), n(x, x, outer=None, ob=x[0, 0]), n(x, x, outer=None, ow=x[0, 0]), n(x, x, scale=x[0]),
+            n(x, x, gate=x[:1]), n(x, x, gate=x[0]), n(x.double(), x.double()), n(x, x, gate=x.half()), n(x, x.half()),
+            n(torch.zeros(1, 16385), torch.zeros(1, 16385)), n(torch.zeros(3, 0), torch.zeros(3, 0)),
+            n(torch.tensor(1.0), torch.tensor(1.0)), n(x, x.to("meta")), n(x, x, inner="rms", iw=x[0, 0, 1:])]
+    muon = [(x[0, 0], 5), (x.double(), 5), (x, 0), (x, 101), (torch.zeros(2, 0, 3), 5), (torch.zeros(2, 3, 0), 5),
+            (x, 5, torch.float64), (x.half(), 5, torch.float32)]
+    return [("gated_feed_forward", a) for a in ffn] + [("residual_norm", a) for a in norm] + [("orthogonalize", a) for a in muon]
+
+
+@pytest.mark.parametrize("at", range(41))
+def test_the_cpu_paths_refuse_what_the_kernels_refuse(at):
+    """With the same words."""
+    from instaorder_amd import gated_feed_forward, layer_ext, orthogonalize, residual_norm
+    name, a = refusals()[at]
+    bind, text = layer_ext.bind(), []
+    if name == "gated_feed_forward":
+        calls = [lambda: bind.gated_feed_forward(*a), lambda: gated_feed_forward(*a)]
+    elif name == "residual_norm":
+        keys = ("gate", "scale", "inner", "inner_weight", "inner_bias", "outer", "outer_weight", "outer_bias", "eps", "want_residual")
+        calls = [lambda: bind.residual_norm(*a), lambda: residual_norm(*a[:2], **dict(zip(keys, a[2:])))]
+    else:
+        calls = [lambda: bind.orthogonalize(a[0], a[1], 1.0, 1.0, 1.0, 1e-7, *a[2:]),
+                 lambda: orthogonalize(a[0], steps=a[1], dtype=a[2] if len(a) > 2 else None)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match=name) as e:
+            call()
+        text.append(str(e.value).split("\n")[0])
+    assert text[0] == text[1] and "Not implemented on the CPU" not in text[0]
+
+
+def test_refusals_are_all_run():
+    assert len(refusals()) == 41
