@@ -73,7 +73,7 @@ int enc_gated_ffn_backward(int dtype, int activation, const void *x, int64_t x_s
  *   n = norm_outer(r)
  *   norm: ENC_NORM_LAYER (v - mean) / sqrt(var + eps) * weight + bias;  ENC_NORM_RMS v / sqrt(mean(v^2) + eps) * weight + bias
  * x, y [rows, width]; gate NULL or [rows / gate_group, width], row i / gate_group belongs to row i (gate_group 1: a gate
- * for each row); scale, weights and biases NULL (absent) or [width].  Width at most 16384; rows need no alignment.
+ * for each row); scale, weights and biases NULL (absent) or [width].  Width at most ENC_NORM_MAX_WIDTH; rows need no alignment.
  * residual: r, may be NULL if there is an outer norm; normed: n, not written without one.  stats: NULL, or 4 floats a
  * row (16-byte aligned) that the backward pass takes.
  * Backward: d_normed is needed with an outer norm; d_residual may be NULL with one and is needed without.  d_x and d_y
@@ -82,6 +82,7 @@ int enc_gated_ffn_backward(int dtype, int activation, const void *x, int64_t x_s
 #define ENC_NORM_NONE 0
 #define ENC_NORM_LAYER 1
 #define ENC_NORM_RMS 2
+#define ENC_NORM_MAX_WIDTH 16384
 
 size_t enc_residual_norm_backward_workspace_bytes(int64_t rows, int64_t width, int64_t gate_group);
 

@@ -8,7 +8,8 @@ hot path of SNU-VGILab/InstaOrder (Mask2Former's MSDeformAttnPixelDecoder encode
   encoder.py          the pixel decoder's MSDA encoder stack, detectron2-free
   pixel_decoder.py    MSDeformAttnPixelDecoder around it (input projections, FPN, mask features)
   layer_ext.py        host side of libenc_hip.so (include/enc_hip.h): operators of the layer around the op
-  layer.py            gated_feed_forward, residual_norm (autograd functions and modules)
+  layer.py            gated_feed_forward, residual_norm: entry points and CPU paths
+  layer_checks.py     their arguments' checks on the CPU
   optim.py            orthogonalize and the Muon optimiser for the stack's weight matrices
   synthetic.py        synthetic inputs of the encoder's shape (bench, tests)
 """

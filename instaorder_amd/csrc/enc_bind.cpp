@@ -20,8 +20,6 @@ using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 typedef std::optional<Tensor> MaybeTensor;
 
-constexpr int64_t NORM_MAX_WIDTH = 16384;
-
 int dtype_code(const char *what, const Tensor &x) {
   switch (x.scalar_type()) {
     case at::kFloat: return ENC_F32;
@@ -225,8 +223,8 @@ struct NormInputs {
 int64_t check_norm(const NormInputs &t, int inner, int outer, bool want_residual) {
   const char *what = "residual_norm";
   dtype_code(what, t.x);
-  TORCH_CHECK(t.x.dim() >= 1 && t.x.size(-1) >= 1 && t.x.size(-1) <= NORM_MAX_WIDTH, what, ": x must be [..., width] with a width of 1 to ",
-              NORM_MAX_WIDTH);
+  TORCH_CHECK(t.x.dim() >= 1 && t.x.size(-1) >= 1 && t.x.size(-1) <= ENC_NORM_MAX_WIDTH, what, ": x must be [..., width] with a width of 1 to ",
+              ENC_NORM_MAX_WIDTH);
   TORCH_CHECK(outer != ENC_NORM_NONE || want_residual, what, ": without an outer norm the residual is the only result");
   const auto shape = t.x.sizes();
   const at::IntArrayRef width = shape.slice(shape.size() - 1);

@@ -13,7 +13,7 @@ import torch
 _bind = None
 
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
-NORM_MAX_WIDTH = 16384
+NORM_MAX_WIDTH = 16384          # ENC_NORM_MAX_WIDTH of the header
 
 
 def bind():

@@ -380,3 +380,12 @@ def test_the_cpu_paths_refuse_what_the_kernels_refuse(at):
 
 def test_refusals_are_all_run():
     assert len(refusals()) == 41
+
+
+def test_the_width_limit_is_one():
+    import os
+    import re
+    from conftest import ROOT
+    from instaorder_amd import layer_ext
+    header = open(os.path.join(ROOT, "include", "enc_hip.h")).read()
+    assert int(re.search(r"#define ENC_NORM_MAX_WIDTH (\d+)", header).group(1)) == layer_ext.NORM_MAX_WIDTH
