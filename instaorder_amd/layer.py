@@ -31,7 +31,7 @@ def gated_feed_forward(x, w_in, b_in, w_out, b_out, activation="silu"):
 
     x [..., width]; w_in [2 * hidden, width] (value rows first, then gate rows -- the order of ``F.glu``); w_out
     [out_width, hidden]; biases may be None.  activation: "silu", "gelu" (by the error function), "sigmoid", "relu".
-    fp32, bf16 or fp16, one type for all; sums are fp32, h is rounded to the type once.  Differentiable once in all five
+    fp32, bf16 or fp16, one type for all; sums are fp32, h is rounded to the type at most once.  Differentiable once in all five
     tensors.  fp32 goes through three bf16 parts in the backward pass and in forward passes of many tokens: there an Inf among
     the inputs gives NaN (its parts multiply zeros), a NaN stays one, and values below 2^-110 lose their low bits (their
     parts end at 2^-133).  Under autocast all five are cast to its type, as for ``F.linear``."""
@@ -41,15 +41,17 @@ def gated_feed_forward(x, w_in, b_in, w_out, b_out, activation="silu"):
     if x.is_cuda:
         return (layer_ext._bind or layer_ext.bind()).gated_feed_forward(x, w_in, b_in, w_out, b_out, activation)
     layer_checks.gated_feed_forward(x, w_in, b_in, w_out, b_out, activation, ACTIVATIONS)
+    dtype = x.dtype                                     # 32 bits inside, one rounding of the result
+    x, w_in, b_in, w_out, b_out = _cast((x, w_in, b_in, w_out, b_out), torch.float32)
     with torch.autocast("cpu", enabled=False):
         a, b = F.linear(x, w_in, b_in).chunk(2, -1)
-        return F.linear(a * ACTIVATIONS[activation](b), w_out, b_out)
+        return F.linear(a * ACTIVATIONS[activation](b), w_out, b_out).to(dtype)
 
 
 def _cpu_norm(v, kind, weight, bias, eps):
     if kind == "layer":
         return F.layer_norm(v, v.shape[-1:], weight, bias, eps)
-    v = v * torch.rsqrt(v.float().pow(2).mean(-1, keepdim=True) + eps).to(v.dtype)
+    v = v * torch.rsqrt(v.pow(2).mean(-1, keepdim=True) + eps)
     v = v if weight is None else v * weight
     return v if bias is None else v + bias
 
@@ -72,7 +74,11 @@ def residual_norm(x, y, *, gate=None, scale=None, inner=None, inner_weight=None,
         return (layer_ext._bind or layer_ext.bind()).residual_norm(x, y, gate, scale, inner, inner_weight, inner_bias, outer,
                                                                    outer_weight, outer_bias, eps, want_residual)
     layer_checks.residual_norm(x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias, want_residual)
+    dtype = x.dtype                                     # 32 bits inside, one rounding of each result
+    x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias = _cast(
+        (x, y, gate, scale, inner_weight, inner_bias, outer_weight, outer_bias), torch.float32)
     z = y if inner is None else _cpu_norm(y, inner, inner_weight, inner_bias, eps)
     z = z if gate is None else z * gate
     r = x + (z if scale is None else z * scale)
-    return r if want_residual else None, None if outer is None else _cpu_norm(r, outer, outer_weight, outer_bias, eps)
+    n = None if outer is None else _cpu_norm(r, outer, outer_weight, outer_bias, eps).to(dtype)
+    return r.to(dtype) if want_residual else None, n

@@ -389,3 +389,34 @@ def test_the_width_limit_is_one():
     from instaorder_amd import layer_ext
     header = open(os.path.join(ROOT, "include", "enc_hip.h")).read()
     assert int(re.search(r"#define ENC_NORM_MAX_WIDTH (\d+)", header).group(1)) == layer_ext.NORM_MAX_WIDTH
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_cpu_paths_round_as_documented(dtype):
+    """16-bit tensors: 32 bits inside and one rounding a result, on the CPU as on the GPU."""
+    import layer_reference as R
+    from instaorder_amd import gated_feed_forward, residual_norm
+    g = torch.Generator().manual_seed(5)
+    r = lambda *s: torch.randn(*s, generator=g).to(dtype)      # noqa: E731
+    t = [v.requires_grad_(True) for v in (r(9, 40), r(48, 40), r(48), r(33, 24), r(33))]
+    grad = r(9, 33)
+    y = gated_feed_forward(*t, activation="gelu")
+    got = dict(zip(("d_x", "d_w_in", "d_b_in", "d_w_out", "d_b_out"), torch.autograd.grad(y, t, grad)), y=y.detach())
+    want = R.ffn(*[v.detach() for v in t], "gelu", grad)
+    assert set(got) == set(want)
+    for k, (v, bound) in want.items():
+        assert got[k].dtype == dtype
+        R.within(got[k], v, bound, k)
+    d = {"x": r(6, 7, 40), "y": r(6, 7, 40), "gate": r(6, 1, 40), "scale": r(40), "inner_weight": r(40), "inner_bias": r(40),
+         "outer_weight": r(40), "outer_bias": r(40)}
+    for inner, outer in (("layer", "rms"), ("rms", "layer")):
+        leaves = {k: v.detach().requires_grad_(True) for k, v in d.items()}
+        res, n = residual_norm(**leaves, inner=inner, outer=outer)
+        grads = {"residual": r(6, 7, 40), "normed": r(6, 7, 40)}
+        got = torch.autograd.grad([res, n], list(leaves.values()), list(grads.values()))
+        got = {"residual": res.detach(), "normed": n.detach(), **{"d_" + k: v for k, v in zip(leaves, got)}}
+        want = R.residual_norm(d, inner, outer, 1e-5, grads)
+        assert set(got) == set(want)
+        for k, w in want.items():
+            # one rounding to the type, and 32-bit sums of at most 64 + 4 sqrt(42) terms of the largest size, spread 16 times
+            R.within(got[k], w, (R.U[dtype] * w.abs()).clamp(min=R.FLOOR[dtype]) + 90 * 16 * R.U32 * (w.abs().max() + 1.0), k)
