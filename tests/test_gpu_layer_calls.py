@@ -51,6 +51,31 @@ def test_gates_shared_over_dimensions_of_one(dtype, lead, gate):
         R.within(v, w, (R.U[dtype] * w.abs()).clamp(min=R.FLOOR[dtype]) + steps * 16 * R.U32 * (size + 1.0) + R.TINY, k)
 
 
+# ---- how h is held ------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m, d, f, o", [(1, 2048, 5632, 2048), (16, 2048, 2056, 520), (7, 1024, 4104, 71), (3, 176, 24600, 64),
+                                        (1, 8200, 520, 8), (16, 64, 96, 64), (1, 1024, 2816, 1024), (5, 33, 17, 41), (16, 2049, 2051, 36)])
+def test_feed_forward_of_few_tokens_holds_the_hidden_values_in_two_parts(dtype, m, d, f, o):
+    """Up to 16 tokens, whatever the weights' size and rows: the result is as good as h were never rounded.
+
+    In the 2-norm a result is off by its own rounding and twice what it is off before (the distance to the next value of a
+    type changes no faster than the value).  Before, it is off by k sums of 32 bits, whose roundings of U32 / sqrt(3) go
+    either way (2.5 sqrt(k) is above four deviations) but for a cut of up to 2 U32 in each matrix instruction of 32 k, and by
+    u^2 of h, what two parts leave over (fp16: or half its smallest step).  One part's rounding of h is as large as y's."""
+    from instaorder_amd import gated_feed_forward
+    args = ffn_inputs(dtype, m, d, f, o, True, seed=m)
+    x, wi, bi, wo, bo = (a.double() for a in args)
+    a, b = (x @ wi.t() + bi).chunk(2, -1)
+    h, u, k = a * R.activate(b, "silu"), R.U[dtype], d + f
+    want = h @ wo.t() + bo
+    size = float((h.square() @ wo.square().t() + bo.square()).sum().sqrt())
+    rest = float(((u * u * h.abs()).clamp(min=R.FLOOR[dtype]).square() @ wo.square().t()).sum().sqrt())
+    tol = float((want.to(dtype).double() - want).norm()) + 2 * ((2.5 * k ** 0.5 + k / 16) * R.U32 * size + rest)
+    leaves = [v.detach().requires_grad_(True) for v in args]                 # and where pre-activations are kept
+    for y in (gated_feed_forward(*args), gated_feed_forward(*leaves).detach()):
+        assert float((y.double() - want).norm()) <= tol
+
+
 # ---- autocast -----------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_operators_under_autocast(dtype):
