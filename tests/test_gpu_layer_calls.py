@@ -76,6 +76,29 @@ def test_feed_forward_of_few_tokens_holds_the_hidden_values_in_two_parts(dtype, 
         assert float((y.double() - want).norm()) <= tol
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m", [5, 100, 700])
+@pytest.mark.parametrize("f", [1, 8, 17, 40])
+def test_feed_forward_infinities_do_not_meet_the_padding(dtype, m, f):
+    """Hidden widths that are no multiple of 8 are padded with zeros, which an Inf would turn to NaN: everything is positive
+    here, so what the definition makes of an Inf is Inf."""
+    from instaorder_amd import gated_feed_forward
+    x, wi, bi, wo, bo = (a.abs() + 0.01 for a in ffn_inputs(dtype, m, 24, f, 16, True))
+    row, rest = m // 2, torch.arange(m, device="cuda") != m // 2
+    clean = gated_feed_forward(x, wi, bi, wo, bo, "relu")
+    x2 = x.clone()
+    x2[row, 3] = float("inf")
+    y = gated_feed_forward(x2, wi, bi, wo, bo, "relu")
+    assert (y[row] == float("inf")).all() and torch.equal(y[rest], clean[rest])
+    leaves = [v.requires_grad_(True) for v in (x, wi, bi, wo, bo)]
+    grad = torch.ones(m, 16, device="cuda", dtype=dtype)
+    grad[row, 5] = float("inf")
+    d_x, d_wi, d_bi, d_wo, d_bo = torch.autograd.grad(gated_feed_forward(*leaves, "relu"), leaves, grad)
+    assert (d_x[row] == float("inf")).all() and d_x[rest].isfinite().all()
+    assert (d_wi == float("inf")).all() and (d_bi == float("inf")).all()
+    assert (d_wo[5] == float("inf")).all() and d_wo[:5].isfinite().all() and d_bo[5] == float("inf")
+
+
 # ---- autocast -----------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_operators_under_autocast(dtype):
