@@ -41,14 +41,56 @@ def test_gates_shared_over_dimensions_of_one(dtype, lead, gate):
     t["gate"] = rand(gen(3), *gate, 72, dtype=dtype)
     got, grads = gradients(t, "layer", "rms")
     want = R.residual_norm(t, "layer", "rms", 1e-5, grads)
+    norm_within(got, want, dtype, t["x"].numel() // 72, 72)
+
+
+def norm_within(got, want, dtype, rows, width):
+    """The bounds of test_gpu_layer.py for rows and column sums; every result and gradient has to be there."""
     assert set(got) == set(want)
-    rows = t["x"].numel() // 72
     for k, v in got.items():
-        # a row's sums are at most 16 + 6 + 16 steps of 32 bits, a column's 64 + 4 sqrt(rows); 16 for the spread of the inputs
         w = want[k]
-        size, steps = (w.abs().amax(-1, keepdim=True), 64) if v.shape == t["x"].shape else (w.abs().max(), 64 + 4 * rows ** 0.5)
-        assert v.shape == w.shape and v.dtype == dtype
+        assert v is not None and v.shape == w.shape and v.dtype == dtype, k
+        row = v.dim() and v.shape[-1] == width and v.numel() == rows * width and v.dim() > 1
+        size, steps = (w.abs().amax(-1, keepdim=True), 64) if row else (w.abs().max(), 64 + 4 * rows ** 0.5)
         R.within(v, w, (R.U[dtype] * w.abs()).clamp(min=R.FLOOR[dtype]) + steps * 16 * R.U32 * (size + 1.0) + R.TINY, k)
+
+
+OPTIONAL = ("gate", "scale", "inner_weight", "inner_bias", "outer_weight", "outer_bias")
+
+
+@pytest.mark.parametrize("present", range(64))
+def test_norm_every_gradient_is_there(present):
+    """Each choice of the optional inputs: all gradients against the 64-bit form, then each input's alone (the scale's is summed
+    in another order where no gate's is formed beside it)."""
+    from instaorder_amd import residual_norm
+    given = [k for i, k in enumerate(OPTIONAL) if present >> i & 1]
+    t = {k: v for k, v in norm_inputs(torch.float32, (3, 7), 40, "layer", "rms", "sample", True, "wb").items() if k in ("x", "y", *given)}
+    got, grads = gradients(t, "layer", "rms")
+    want = R.residual_norm(t, "layer", "rms", 1e-5, grads)
+    norm_within(got, want, torch.float32, 21, 40)
+    for k in t:
+        one = {n: v.detach().requires_grad_(n == k) for n, v in t.items()}
+        r, n = residual_norm(**one, inner="layer", outer="rms")
+        v, = torch.autograd.grad([r, n], one[k], list(grads.values()))
+        norm_within({"d_" + k: v}, {"d_" + k: want["d_" + k]}, torch.float32, 21, 40)
+
+
+@pytest.mark.parametrize("present", range(4))
+def test_feed_forward_every_gradient_is_there(present):
+    from instaorder_amd import gated_feed_forward
+    args = ffn_inputs(torch.float32, 70, 40, 48, 24, True)
+    args[2], args[4] = args[2] if present & 1 else None, args[4] if present & 2 else None
+    grad = rand(gen(5), 70, 24)
+    want = R.ffn(*args, "silu", grad)
+    names = ("d_x", "d_w_in", "d_b_in", "d_w_out", "d_b_out")
+    leaves = [None if a is None else a.detach().requires_grad_(True) for a in args]
+    all_of = [(i, v) for i, v in enumerate(leaves) if v is not None]
+    got = torch.autograd.grad(gated_feed_forward(*leaves), [v for _, v in all_of], grad)
+    for (i, _), v in zip(all_of, got):
+        R.within(v, *want[names[i]], names[i])
+        one = [None if a is None else a.detach().requires_grad_(j == i) for j, a in enumerate(args)]
+        alone, = torch.autograd.grad(gated_feed_forward(*one), one[i], grad)
+        assert torch.equal(alone, v), names[i]
 
 
 # ---- how h is held ------------------------------------------------------------------------------
