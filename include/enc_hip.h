@@ -32,6 +32,10 @@ extern "C" {
 #define ENC_F16 2
 /* enc_orthogonalize and its workspace query: | ENC_BF16 or ENC_F16, the result's type, of an update in fp32 */
 #define ENC_UPDATE_F32 16
+/* the workspace queries of the feed-forward block: | the dtype, for a call whose tensors can be read where they lie: every
+ * address a multiple of 16 bytes, every row stride a multiple of 8 elements and below 2^22.  Without it there is room to lay
+ * all of them out, which is enough for any call. */
+#define ENC_IN_PLACE 32
 
 #define ENC_ACT_SILU 0
 #define ENC_ACT_GELU 1 /* x * Phi(x), by the error function */

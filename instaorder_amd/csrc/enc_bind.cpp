@@ -138,6 +138,10 @@ FfnSizes check_ffn(const Tensor &x, const Tensor &w_in, const Tensor &b_in, cons
   return s;
 }
 
+// The workspace query's type: can the tensors be read where they lie?
+bool aligned16(const Tensor &t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0; }
+bool lies_well(const Rows &r) { return aligned16(r.t) && r.stride % 8 == 0 && r.stride < ((int64_t)1 << 22); }
+
 Tensor ffn_forward(const Tensor &x, const Tensor &w_in, const Tensor &b_in, const Tensor &w_out, const Tensor &b_out, int act, Tensor *pre) {
   const char *what = "gated_feed_forward";
   not_traced(what);
@@ -152,7 +156,8 @@ Tensor ffn_forward(const Tensor &x, const Tensor &w_in, const Tensor &b_in, cons
   shape.back() = s.out_width;
   const Tensor y = at::empty(shape, x.options().requires_grad(false));
   if (pre) *pre = at::empty({(int64_t)enc_gated_ffn_pre_floats(tokens, s.hidden)}, x.options().dtype(at::kFloat).requires_grad(false));
-  const size_t bytes = enc_gated_ffn_forward_workspace_bytes(code, tokens, s.width, s.hidden, s.out_width);
+  const int placed = lies_well(rows) && aligned16(wi) && aligned16(wo) ? ENC_IN_PLACE : 0;
+  const size_t bytes = enc_gated_ffn_forward_workspace_bytes(code | placed, tokens, s.width, s.hidden, s.out_width);
   const Tensor ws = workspace(bytes, x);
   done(what, enc_gated_ffn_forward(code, act, ptr(rows.t), rows.stride, ptr(wi), ptr(bi), ptr(wo), ptr(bo), tokens, s.width, s.hidden,
                                    s.out_width, ptr(y), pre ? pre->data_ptr<float>() : nullptr, ptr(ws), bytes, stream_of(x)));
@@ -190,7 +195,8 @@ struct GatedFeedForward : public torch::autograd::Function<GatedFeedForward> {
     variable_list out(6);
     for (int i = 0; i < 5; ++i)
       if (needs(ctx, i)) out[i] = at::empty(shapes[i], options);
-    const size_t bytes = enc_gated_ffn_backward_workspace_bytes(code, tokens, width, hidden, out_width);
+    const int placed = lies_well(rows) && lies_well(g) && aligned16(wi) && aligned16(wo) ? ENC_IN_PLACE : 0;
+    const size_t bytes = enc_gated_ffn_backward_workspace_bytes(code | placed, tokens, width, hidden, out_width);
     const Tensor ws = workspace(bytes, x);
     done(what, enc_gated_ffn_backward(code, (int)ctx->saved_data["act"].toInt(), ptr(rows.t), rows.stride, ptr(wi), ptr(wo),
                                       pre.data_ptr<float>(), ptr(g.t), g.stride, tokens, width, hidden, out_width, ptr(out[0]), ptr(out[1]),

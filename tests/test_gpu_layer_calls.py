@@ -93,6 +93,30 @@ def test_feed_forward_every_gradient_is_there(present):
         assert torch.equal(alone, v), names[i]
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_feed_forward_takes_no_room_for_copies_that_it_does_not_make(dtype):
+    """A training call whose tensors lie well: beside its results and what it saves (a, b in 32 bits) it holds h, its gradients,
+    and sums.  The same call on rows that have to be laid out gives the same."""
+    from instaorder_amd import gated_feed_forward
+    m, d, f = 1024, 2048, 2048
+    args = [a.requires_grad_(True) for a in ffn_inputs(dtype, m, d, f, d, True)]
+    grad = rand(gen(2), m, d, dtype=dtype)
+    y = gated_feed_forward(*args)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = torch.autograd.grad(y, args, grad)
+    peak = torch.cuda.max_memory_allocated() - before
+    results = sum(g.numel() for g in got) * 2
+    hidden = 3 * m * f * 2                              # h, da, db
+    # sums: slices of k in 32 bits (their number grows until the chip is full: 512 tiles of 128 x 128 at most), 64 rows of columns
+    assert peak <= results + hidden + 4 * (512 * 128 * 128 + 64 * 2 * f) + (1 << 20)
+    shifted = [torch.cat((torch.zeros(1, device="cuda", dtype=dtype), a.detach().flatten()))[1:].view(a.shape).requires_grad_(True) for a in args]
+    y2 = gated_feed_forward(*shifted)
+    again = torch.autograd.grad(y2, shifted, grad)
+    assert torch.equal(y, y2) and all(torch.equal(a, b) for a, b in zip(got, again))
+
+
 # ---- how h is held ------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("m, d, f, o", [(1, 2048, 5632, 2048), (16, 2048, 2056, 520), (7, 1024, 4104, 71), (3, 176, 24600, 64),

@@ -420,3 +420,35 @@ def test_cpu_paths_round_as_documented(dtype):
         for k, w in want.items():
             # one rounding to the type, and 32-bit sums of at most 64 + 4 sqrt(42) terms of the largest size, spread 16 times
             R.within(got[k], w, (R.U[dtype] * w.abs()).clamp(min=R.FLOOR[dtype]) + 90 * 16 * R.U32 * (w.abs().max() + 1.0), k)
+
+
+@pytest.mark.parametrize("backward", [False, True])
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_workspace_of_calls_whose_tensors_lie_well(dtype, backward):
+    """Room for copies is asked for only where copies are made: the query's flag, what a call then needs, and its refusal of a
+    workspace of that size where a tensor has to be laid out after all.  (Launches fail without a device, or are not reached.)"""
+    from test_layer_cpu import lib
+    handle, m, d, f, o = lib(), 512, 64, 256, 72
+    query = handle.enc_gated_ffn_backward_workspace_bytes if backward else handle.enc_gated_ffn_forward_workspace_bytes
+    full, placed = query(dtype, m, d, f, o), query(dtype | 32, m, d, f, o)
+    copies = 2 * (m * d + 2 * f * d + o * f + (m * o if backward else 0))
+    assert full - placed == (copies if dtype else 0)                          # (fp32 is laid out in parts in any case)
+    assert query(9 | 32, m, d, f, o) == 0
+    odd = query(dtype, m, d, f + 1, o) - query(dtype | 32, m, d, f + 1, o)     # odd hidden widths: the weights are laid out
+    assert odd == (2 * (m * d + (m * o if backward else 0)) if dtype else 0)
+
+    def call(nbytes, **change):
+        a = {**dict(x=256, ld=d, w_in=256, w_out=256, grad=256, grad_ld=o), **change}
+        if backward:
+            return handle.enc_gated_ffn_backward(dtype, 0, a["x"], a["ld"], a["w_in"], a["w_out"], 256, a["grad"], a["grad_ld"], m, d, f, o,
+                                                 256, 256, 256, 256, 256, 256, nbytes, None)
+        return handle.enc_gated_ffn_forward(dtype, 0, a["x"], a["ld"], a["w_in"], None, a["w_out"], None, m, d, f, o, 256, None, 256,
+                                            nbytes, None)
+
+    assert call(placed - 1) == 1 and "workspace" in handle.enc_last_error().decode()
+    if dtype:
+        for change in (dict(x=258), dict(ld=d + 1), dict(ld=1 << 22), dict(w_in=264), dict(w_out=266),
+                       *([dict(grad=258), dict(grad_ld=o + 4)] if backward else [])):
+            assert call(placed, **change) == 1 and "workspace" in handle.enc_last_error().decode(), change
+    if not torch.cuda.is_available():
+        assert call(placed) == 2 and call(full, x=264) == 2
