@@ -164,8 +164,9 @@ Tensor ffn_forward(const Tensor &x, const Tensor &w_in, const Tensor &b_in, cons
   return y;
 }
 
-// Saves x, the two weights and the pre-activations in fp32 (8 bytes a hidden value, what a 16-bit eager block keeps in
-// four tensors), so that the gradients are formed from unrounded values.
+// Saves x, the two weights and the pre-activations a, b in fp32 (8 bytes a hidden value, what a 16-bit eager block keeps in
+// four tensors): activation, slope, h, da and db are formed from unrounded values, and the last three rounded to the type
+// once, where they become operands.
 struct GatedFeedForward : public torch::autograd::Function<GatedFeedForward> {
   static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w_in, const MaybeTensor &b_in, const Tensor &w_out,
                         const MaybeTensor &b_out, int64_t act) {
