@@ -80,10 +80,11 @@ void done(const char *what, int rc) { TORCH_CHECK(rc == ENC_OK, what, ": ", enc_
 void on_gpu(const Tensor &x) { TORCH_CHECK(x.is_cuda(), "Not implemented on the CPU"); }
 
 // A trace records torch's own operators: of a call here it would keep the allocation of the result and lose the launch that
-// fills it.
+// fills it.  Under a mode of fake tensors there is no memory to launch on.
 void not_traced(const char *what) {
-  TORCH_CHECK(!torch::jit::tracer::isTracing() &&
-                  !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY),
+  typedef c10::impl::TorchDispatchModeTLS Modes;
+  TORCH_CHECK(!torch::jit::tracer::isTracing() && !Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY) &&
+                  !Modes::get_mode(c10::impl::TorchDispatchModeKey::FAKE),
               what, ": cannot be traced (the trace would not hold the kernels)");
 }
 

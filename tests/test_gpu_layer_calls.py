@@ -247,6 +247,28 @@ def test_traced_layer_takes_its_modules(activation):
             assert torch.allclose(traced(x), call(x), atol=1e-4)
 
 
+def test_compiled_and_inference_mode_calls_are_the_eager_ones():
+    """torch.compile breaks its graph at the kernels."""
+    import warnings
+    from instaorder_amd import gated_feed_forward, residual_norm
+    x, wi, bi, wo, bo = ffn_inputs(torch.float32, 9, 16, 24, 16, True)
+
+    def call(x):
+        return gated_feed_forward(residual_norm(x, x * 2, outer="rms")[1], wi, bi, wo, bo) + 1
+
+    want = call(x)
+    with torch.inference_mode():
+        assert torch.equal(call(x), want)
+    y = x.clone().requires_grad_(True)
+    d_want, = torch.autograd.grad(call(y).sum(), y)
+    with warnings.catch_warnings():
+        warnings.simplefilter("ignore")
+        compiled = torch.compile(call, backend="aot_eager")
+        assert torch.equal(compiled(x), want)
+        d, = torch.autograd.grad(compiled(y).sum(), y)
+    assert torch.equal(d, d_want)
+
+
 # ---- Muon ---------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype, size", [(torch.float16, 9000.0), (torch.float16, 1.0), (torch.float16, 1e-5), (torch.float16, 2e-7),
                                          (torch.bfloat16, 1e30), (torch.bfloat16, 1.0)])

@@ -452,3 +452,11 @@ def test_workspace_of_calls_whose_tensors_lie_well(dtype, backward):
             assert call(placed, **change) == 1 and "workspace" in handle.enc_last_error().decode(), change
     if not torch.cuda.is_available():
         assert call(placed) == 2 and call(full, x=264) == 2
+
+
+@pytest.mark.parametrize("name", ["gated_feed_forward", "residual_norm", "orthogonalize"])
+def test_fake_tensors_are_refused(name):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    call, x = raw_calls()[name], torch.randn(4, 8)
+    with FakeTensorMode() as mode, pytest.raises(RuntimeError, match=name + ".*cannot be traced"):
+        call(mode.from_tensor(x))
