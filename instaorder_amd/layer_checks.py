@@ -1,5 +1,8 @@
 """Checks of the layer operators' arguments for their CPU paths: what the compiled binding (csrc/enc_bind.cpp) checks for GPU
-tensors, with the same words, so that CPU tensors need no build."""
+tensors, with the same words, so that CPU tensors need no build.  Under torch.jit.trace, where sizes are values of the trace and
+asking about them is not, nothing is checked beyond what torch's own operators check."""
+import functools
+
 import torch
 
 from .layer_ext import DTYPES, NORM_MAX_WIDTH
@@ -10,8 +13,20 @@ def _require(condition, text, *args):
         raise RuntimeError(text % args)
 
 
+_NAMES = {torch.float32: "Float", torch.float64: "Double", torch.float16: "Half", torch.bfloat16: "BFloat16", torch.bool: "Bool",
+          torch.uint8: "Byte", torch.int8: "Char", torch.int16: "Short", torch.int32: "Int", torch.int64: "Long"}
+
+
 def _name(dtype):
-    return torch.empty(0, dtype=dtype).type().split(".")[-1][:-len("Tensor")]
+    return _NAMES.get(dtype, str(dtype))
+
+
+def _not_while_tracing(check):
+    @functools.wraps(check)
+    def checked(*args):
+        if not torch.jit.is_tracing():
+            check(*args)
+    return checked
 
 
 def _type(what, x):
@@ -27,6 +42,7 @@ def _like(what, x, name, t, shape):
     _require(list(t.shape) == list(shape), "%s: %s has shape %s, not %s", what, name, list(t.shape), list(shape))
 
 
+@_not_while_tracing
 def gated_feed_forward(x, w_in, b_in, w_out, b_out, activation, activations):
     what = "gated_feed_forward"
     _require(activation in activations, "%s: unknown activation '%s' (one of %s)", what, activation, ", ".join(sorted(activations)))
@@ -40,6 +56,7 @@ def gated_feed_forward(x, w_in, b_in, w_out, b_out, activation, activations):
         _like(what, x, name, t, shape)
 
 
+@_not_while_tracing
 def residual_norm(x, y, gate, scale, inner, inner_weight, inner_bias, outer, outer_weight, outer_bias, want_residual):
     what = "residual_norm"
     for kind in (inner, outer):

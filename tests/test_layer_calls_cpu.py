@@ -460,3 +460,21 @@ def test_fake_tensors_are_refused(name):
     call, x = raw_calls()[name], torch.randn(4, 8)
     with FakeTensorMode() as mode, pytest.raises(RuntimeError, match=name + ".*cannot be traced"):
         call(mode.from_tensor(x))
+
+
+def test_cpu_paths_can_be_traced():
+    """They are torch's own operators; the checks leave nothing in the trace, whatever they look at."""
+    import warnings
+    from instaorder_amd import gated_feed_forward, residual_norm
+    wi, wo, gate, w = torch.randn(12, 8), torch.randn(8, 6), torch.randn(2, 1, 8), torch.randn(8)
+
+    def call(x):
+        r, n = residual_norm(x, 2 * x, gate=gate, outer="rms", outer_weight=w)
+        return gated_feed_forward(n, wi, None, wo, None), r
+
+    with warnings.catch_warnings():
+        warnings.simplefilter("error", torch.jit.TracerWarning)
+        traced = torch.jit.trace(call, torch.randn(2, 3, 8))
+    x = torch.randn(2, 3, 8)
+    assert all(torch.allclose(a, b) for a, b in zip(traced(x), call(x)))
+    assert "aten::empty" not in str(traced.graph)
