@@ -74,11 +74,24 @@ inline int pick_group(int D) {
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// spatial_size == 0 with queries: no level can lie inside the value tensor, every sample reads zero
-int zero_output(const char *who, void *out, size_t bytes, hipStream_t st) {
-  const hipError_t e = hipMemsetAsync(out, 0, bytes, st);
-  if (e != hipSuccess) return fail(MSDA_ERR_LAUNCH, "%s: hipMemsetAsync(output) failed: %s", who, hipGetErrorString(e));
-  return MSDA_OK;
+// Zeros `bytes` bytes.  A kernel, not hipMemsetAsync: in a captured graph the memset's node has left values of an earlier replay
+// standing (a generic backward of 24 channels a head, replayed on new data: 1e27 in grad_value).
+__global__ __launch_bounds__(256) void msda_zero_kernel(uint8_t *p, size_t head, size_t chunks, size_t tail) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const size_t i0 = (size_t)blockIdx.x * 256 + threadIdx.x;
+  u32x4 *q = reinterpret_cast<u32x4 *>(p + head);
+  for (size_t i = i0; i < chunks; i += (size_t)gridDim.x * 256) q[i] = u32x4{0u, 0u, 0u, 0u};
+  if (i0 < head) p[i0] = 0;
+  if (i0 < tail) p[head + chunks * 16 + i0] = 0;
+}
+int zero_memory(const char *who, void *out, size_t bytes, hipStream_t st) {
+  if (bytes == 0) return MSDA_OK;
+  size_t head = (16 - (reinterpret_cast<uintptr_t>(out) & 15u)) & 15u;
+  if (head > bytes) head = bytes;
+  const size_t chunks = (bytes - head) / 16, blocks = (chunks + 255) / 256;
+  launch(msda_zero_kernel, dim3((unsigned)(blocks < 1 ? 1 : blocks < 4096 ? blocks : 4096)), dim3(256), 0, st, static_cast<uint8_t *>(out),
+         head, chunks, (bytes - head) & 15u);
+  return check_launch(who);
 }
 
 template <typename T>
@@ -235,12 +248,7 @@ int backward_atomic(const char *who, const T *value, const int64_t *shapes, cons
                     int L, int Lq, int P, T *grad_value, T *grad_loc, T *grad_aw,
                     hipStream_t st) {
   const size_t vbytes = sizeof(T) * (size_t)N * S * M * D;
-  if (vbytes) {
-    const hipError_t e = hipMemsetAsync(grad_value, 0, vbytes, st);
-    if (e != hipSuccess)
-      return fail(MSDA_ERR_LAUNCH, "%s: hipMemsetAsync(grad_value) failed: %s", who,
-                  hipGetErrorString(e));
-  }
+  if (int rc = zero_memory(who, grad_value, vbytes, st)) return rc;
   if ((size_t)N * Lq == 0) return MSDA_OK;
   return backward_generic<T>(value, shapes, lsi, loc, aw, grad_out, N, S, M, D, L, Lq, P,
                              grad_value, grad_loc, grad_aw, st);
@@ -417,9 +425,7 @@ int launch_binned_group(const char *who, const VT *value, const int64_t *shapes,
   if (split) {
     sums = GV16 ? reinterpret_cast<float *>(static_cast<char *>(workspace) + staging_off)
                 : reinterpret_cast<float *>(grad_value);
-    const hipError_t e = hipMemsetAsync(sums, 0, sizeof(float) * gv_elems, st);
-    if (e != hipSuccess)
-      return fail(MSDA_ERR_LAUNCH, "%s: hipMemsetAsync(grad_value) failed: %s", who, hipGetErrorString(e));
+    if (int rc = zero_memory(who, sums, sizeof(float) * gv_elems, st)) return rc;
   }
   // one scatter pass + one tile-kernel pass per round (one round unless the caller's workspace is short); a round
   // without lists returns at once
@@ -589,7 +595,7 @@ int backward_f32_noalloc(const char *who, const float *value, const int64_t *sha
   if (int rc = check_dims(who, N, S, M, D, L, Lq, P)) return rc;
   const bool fast = binned_shape(N, S, M, D, L, Lq, P) && aligned16(value) && aligned16(grad_out) &&
                     aligned16(grad_value) && aligned16(loc) && aligned16(grad_loc) && bwd_impl_choice() != 0;
-  if (!fast)   // the generic kernels use no scratch buffer at all (one hipMemsetAsync, no allocation)
+  if (!fast)   // the generic kernels use no scratch buffer at all (grad_value is cleared by a kernel)
     return backward_atomic<float>(who, value, shapes, lsi, loc, aw, grad_out, N, S, M, D, L, Lq, P, grad_value,
                                   grad_loc, grad_aw, static_cast<hipStream_t>(stream));
   // the batch goes through the built-in array in groups of as many images as fit (images are independent)
@@ -646,7 +652,7 @@ int fused_forward(const char *who, const VT *value, const int64_t *shapes, const
     return fail(MSDA_ERR_INVALID_ARGUMENT,
                 "%s: needs channels == 32, num_levels * num_point <= %d, aligned tensors of < 2^30 "
                 "elements (use the unfused entry points otherwise)", who, FWD_FUSED_MAX_LP);
-  if (S == 0) return zero_output(who, out, npairs * 32 * sizeof(VT), static_cast<hipStream_t>(stream));
+  if (S == 0) return zero_memory(who, out, npairs * 32 * sizeof(VT), static_cast<hipStream_t>(stream));
   constexpr uint32_t GP = 64u / FwdLanes<VT>::LPG;
   const size_t lds = (size_t)4 * ((size_t)2 * GP * (size_t)(L * P + 1) * 16 + (((size_t)GP * L * P + 3) / 4) * 16);
   const uint32_t nq = (uint32_t)((size_t)N * Lq), nunits = ((nq + GP - 1u) / GP) * (uint32_t)M;
@@ -889,7 +895,7 @@ int msda_forward_bf16(const uint16_t *value, const int64_t *spatial_shapes,
       (reinterpret_cast<uintptr_t>(output) & 7u))
     return fail(MSDA_ERR_INVALID_ARGUMENT,
                 "msda_forward_bf16: needs channels == 32, 8-byte aligned tensors of < 2^30 elements");
-  if (S == 0) return zero_output("msda_forward_bf16", output, npairs * 32 * sizeof(uint16_t), static_cast<hipStream_t>(stream));
+  if (S == 0) return zero_memory("msda_forward_bf16", output, npairs * 32 * sizeof(uint16_t), static_cast<hipStream_t>(stream));
   launch_forward_d32<bf16_t>(reinterpret_cast<const bf16_t *>(value), spatial_shapes,
                              level_start_index, sampling_loc, attn_weight, S, M, L, Lq, P, npairs,
                              reinterpret_cast<bf16_t *>(output), static_cast<hipStream_t>(stream));
