@@ -31,9 +31,8 @@ def gated_feed_forward(x, w_in, b_in, w_out, b_out, activation="silu"):
 
     x [..., width]; w_in [2 * hidden, width] (value rows first, then gate rows -- the order of ``F.glu``); w_out
     [out_width, hidden]; biases may be None.  activation: "silu", "gelu" (by the error function), "sigmoid", "relu".
-    fp32, bf16 or fp16, one type for all; sums are fp32, h is rounded to the type at most once (up to 16
-    tokens it is held in twice the type's bits).  Differentiable once in all five
-    tensors.  fp32 goes through three bf16 parts in the backward pass and in forward passes of many tokens: there an Inf among
+    fp32, bf16 or fp16, one type for all; sums are fp32, h is rounded to the type at most once (up to 16 tokens it is held in
+    two parts of the type, so that there an Inf in w_out gives NaN).  Differentiable once in all five tensors.  fp32 goes through three bf16 parts in the backward pass and in forward passes of many tokens: there an Inf among
     the inputs gives NaN (its parts multiply zeros), a NaN stays one, and values below 2^-110 lose their low bits (their
     parts end at 2^-133).  Under autocast all five are cast to its type, as for ``F.linear``."""
     dtype = autocast_dtype(x)
